@@ -236,6 +236,51 @@ int vings_sparse_adam_multi(int n_groups, float* const* params_host,
                             const float* lrs_host, const uint8_t* visible, float b1, float b2,
                             float eps, int N, void* stream);
 
+/* The same update on gradients clipped by their global norm:
+ *   norm = sqrt(sum over all groups and visible rows of g^2)
+ *   g' = g * min(1, max_norm / (norm + 1e-6)), then the update above on g'
+ * Gradients of invisible rows count in nothing and invisible elements are not written.  A norm
+ * that is infinite or NaN skips the step on the device: parameters and moments stay.  `norm`
+ * (device, one float) receives the norm before clipping in every case.  Up to 64 groups, each
+ * with its own b1, b2 and eps; arrays need 4-byte alignment only.  `instance_count` (may be
+ * NULL) and `capacity`: as in vings_sparse_adam_multi_guarded.  The workspace holds the partial
+ * sums of the norm; nothing in it outlives the call. */
+size_t vings_sparse_adam_clipped_workspace_bytes(int n_groups);
+int vings_sparse_adam_clipped(int n_groups, float* const* params_host, const float* const* grads_host,
+                              float* const* exp_avgs_host, float* const* exp_avg_sqs_host,
+                              const int* widths_host, const float* lrs_host, const float* b1s_host,
+                              const float* b2s_host, const float* epss_host, const uint8_t* visible,
+                              int N, float max_norm, float* norm, void* workspace,
+                              size_t workspace_bytes, const uint32_t* instance_count,
+                              uint32_t capacity, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Element types of the entry points that take more than float32. */
+#define VINGS_F32 0
+#define VINGS_BF16 1
+#define VINGS_F16 2
+
+/* ------------------------------------------------------------------------
+ * Global norm of many gradient tensors, and clipping by it (the reference limits the gradients
+ * of its tracker network between backward and the optimiser, frontend/modules/clipping.py).
+ *   norm_kind 0: norm = sqrt(sum of squares over all tensors), 1: the largest magnitude
+ *   clip: out = g * min(1, max_norm / (norm + 1e-6)), rounded once to the type of out
+ * The lists live in HOST memory and are read before the call returns; tensors may be empty, of
+ * different types and aligned to their element only.  Any number of tensors; sums are held in
+ * 64 bits and joined in a fixed order.  `norm`: one float on the device, written in every case
+ * (0 for empty lists); a NaN among the gradients gives a NaN norm, and NaN clipped gradients;
+ * an infinity gives an infinite norm and the coefficient 0.
+ * vings_grad_clip: outs[i] is grads[i] itself (in place; nothing is written when the coefficient
+ * is 1) or memory that overlaps no other tensor of the call; its type is grads[i]'s or float32. */
+size_t vings_grad_norm_workspace_bytes(int n_tensors, const int64_t* numels_host);
+int vings_grad_norm(int n_tensors, const void* const* grads_host, const int64_t* numels_host,
+                    const int* types_host, int norm_kind, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int vings_grad_clip(int n_tensors, const void* const* grads_host, void* const* outs_host,
+                    const int64_t* numels_host, const int* types_host, const int* out_types_host,
+                    int norm_kind, float max_norm, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Parameter activations of get_property (gaussian_base.py:44-48,64-72):
  * opacity = sigmoid(raw), scaling = exp(raw), rotation = raw / max(|raw|, 1e-12)

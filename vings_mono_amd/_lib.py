@@ -3,6 +3,7 @@
 There is no CPU fallback: if the shared object is missing or a call fails the
 caller gets an exception.
 """
+import contextlib
 import ctypes
 import os
 
@@ -51,6 +52,12 @@ _SIGNATURES = {
     "vings_sparse_adam": (_c.c_int, [_P] * 5 + [_c.c_float] * 4 + [_c.c_int, _c.c_int, _P]),
     "vings_sparse_adam_multi": (_c.c_int, [_c.c_int] + [_P] * 7 + [_c.c_float] * 3 +
                                 [_c.c_int, _P]),
+    "vings_sparse_adam_clipped_workspace_bytes": (_c.c_size_t, [_c.c_int]),
+    "vings_sparse_adam_clipped": (_c.c_int, [_c.c_int] + [_P] * 10 + [_c.c_int, _c.c_float, _P, _P,
+                                                                      _c.c_size_t, _P, _c.c_uint32, _P]),
+    "vings_grad_norm_workspace_bytes": (_c.c_size_t, [_c.c_int, _P]),
+    "vings_grad_norm": (_c.c_int, [_c.c_int] + [_P] * 3 + [_c.c_int, _P, _P, _c.c_size_t, _P]),
+    "vings_grad_clip": (_c.c_int, [_c.c_int] + [_P] * 5 + [_c.c_int, _c.c_float, _P, _P, _c.c_size_t, _P]),
     "vings_splat_activate": (_c.c_int, [_c.c_int] + [_P] * 7),
     "vings_surfel_project_backward_finish": (_c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.c_float] +
                                              [_P] * 14 + [_c.c_int64, _c.c_int] + [_P] * 10),
@@ -156,6 +163,17 @@ def ptr(t):
 
 def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # VINGS_F32, _BF16, _F16
+
+
+def on_device(device):
+    """Context in which kernels are launched for tensors of `device`: that device is made current
+    for the call if it is not."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_gpu_tensor(t, name, dtype=None):

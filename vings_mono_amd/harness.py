@@ -240,8 +240,14 @@ class SurfelMapper:
 
     NAMES = ("_xyz", "_rgb", "_opacity", "_scaling", "_rotation")
 
-    def __init__(self, raw_params, device, lr=DEFAULT_LR, loss_weights=DEFAULT_LOSS_WEIGHTS):
+    def __init__(self, raw_params, device, lr=DEFAULT_LR, loss_weights=DEFAULT_LOSS_WEIGHTS,
+                 max_grad_norm=None):
+        """`max_grad_norm`: every view step clips its gradients by their global norm over the
+        splats it steps (SparseGaussianAdam.step(max_norm=)); `last_grad_norm` is the norm of the
+        latest step before clipping, a device scalar."""
         self.device = torch.device(device)
+        self.max_grad_norm = max_grad_norm
+        self.last_grad_norm = None
         self.params = {k: torch.nn.Parameter(raw_params[k].to(self.device).float().contiguous())
                        for k in self.NAMES}
         n = self.params["_xyz"].shape[0]
@@ -328,7 +334,7 @@ class SurfelMapper:
             self.globalkf_max_scores = torch.where(replace, s0, self.globalkf_max_scores)
             self.globalkf_id = torch.where(replace, torch.full_like(self.globalkf_id, kf_id),
                                            self.globalkf_id)
-        self.optimizer.step(vis, self.n)
+        self.last_grad_norm = self.optimizer.step(vis, self.n, max_norm=self.max_grad_norm)
         # (gaussian_base.py:403 calls zero_grad() with torch's default, which drops the gradient
         # tensors: the next backward assigns fresh ones instead of filling and adding)
         self.optimizer.zero_grad()
@@ -407,6 +413,9 @@ class SurfelMapper:
         mapping loss never reads) where the default takes the lean ones."""
         from . import _lib, surfel
         L = _lib.lib()
+        if self.max_grad_norm is not None and reducer is not None and reducer.world > 1 and reducer.compact:
+            raise _lib.VingsError("max_grad_norm needs the whole gradient before the step; the compact "
+                                  "exchange applies it chunk by chunk: use a reducer with compact=False")
         self._match_reducer(reducer)
         fb = self._fused_buffers()
         P, n, dev = self.params, self.n, self.device
@@ -457,7 +466,7 @@ class SurfelMapper:
                     _lib.check(L.vings_splat_unpack_exchange(
                         n, ptr(reducer.fbuf), ptr(self.global_scores), ptr(self.local_scores),
                         *grad_ptrs, ptr(vis), stream), "vings_splat_unpack_exchange")
-                self.optimizer.step(vis, n)
+                self.last_grad_norm = self.optimizer.step(vis, n, max_norm=self.max_grad_norm)
         self.last_loss = loss_vec[0]
         self.last_loss_terms = loss_vec
         self._last_radii = st.radii
@@ -498,8 +507,9 @@ class SurfelMapper:
                 int(kf_id), ptr(g["_xyz"]), ptr(g["_rgb"]), ptr(g["_opacity"]), ptr(g["_scaling"]),
                 ptr(g["_rotation"]), ptr(fb["vis"]), count_ptr, int(capacity), stream),
                 "vings_surfel_project_backward_finish_guarded")
-            self.optimizer.step(fb["vis"], n, guard=(count_ptr, capacity))
-        return loss_vec, st
+            norm = self.optimizer.step(fb["vis"], n, guard=(count_ptr, capacity),
+                                       max_norm=self.max_grad_norm)
+        return loss_vec, st, norm
 
     def drop_view_graphs(self):
         """Forget the captured view steps (and give their memory pool back): the arrays they
@@ -511,7 +521,7 @@ class SurfelMapper:
         """Everything a captured view step has baked in by address: a change (map maintenance
         replaces the parameter and moment arrays, a new keyframe brings new images) makes the
         graph stale."""
-        sig = [self.n, self.stable_skip]
+        sig = [self.n, self.stable_skip, self.max_grad_norm]
         for k in self.NAMES:
             p = self.params[k]
             st = self.optimizer.state.get(p, {})
@@ -575,16 +585,17 @@ class SurfelMapper:
             g = torch.cuda.CUDAGraph()
             torch.cuda.synchronize(self.device)
             with torch.cuda.graph(g, pool=pool):
-                loss_vec, st = self._fused_view_fixed(settings, intr, gt, Rw2c_host, kf_id, cap, count)
+                loss_vec, st, norm = self._fused_view_fixed(settings, intr, gt, Rw2c_host, kf_id, cap, count)
             if pool is None:
                 self._view_graph_pool = g.pool()       # the graphs of a window share their memory
-            ent.update(graph=g, capacity=cap, count=count, loss=loss_vec, radii=st.radii,
+            ent.update(graph=g, capacity=cap, count=count, loss=loss_vec, radii=st.radii, grad_norm=norm,
                        event=torch.cuda.Event(), retired=None)
         ent["graph"].replay()
         ent["event"].record()
         self.last_loss = ent["loss"][0]
         self.last_loss_terms = ent["loss"]
         self._last_radii = ent["radii"]
+        self.last_grad_norm = ent["grad_norm"]
         return ent["loss"]
 
     _WIDTHS = (3, 3, 1, 2, 4)

@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import check, ptr, stream_ptr
+from .gradients import norm_and_workspace
 
 GEOM_STRIDE = 24
 GRAD_STRIDE = 20
@@ -529,14 +530,22 @@ class SparseGaussianAdam(torch.optim.Adam):
                 (ctypes.c_float * n)(*lrs), b1, b2, eps)
 
     @torch.no_grad()
-    def step(self, visibility, N, guard=None):
+    def step(self, visibility, N, guard=None, max_norm=None):
         """`guard` = (device address of a view's instance count, capacity): the step does
-        nothing if the count exceeds the capacity (vings_sparse_adam_multi_guarded)."""
+        nothing if the count exceeds the capacity (vings_sparse_adam_multi_guarded).
+
+        `max_norm`: the gradients are clipped by their global norm over the visible rows of all
+        groups, scaled by min(1, max_norm / (norm + 1e-6)) inside the update (the .grad tensors
+        are not written), and the norm before clipping is returned as a device scalar.  A norm
+        that is infinite or NaN skips the step: parameters and moments stay
+        (vings_sparse_adam_clipped).  Without max_norm nothing is returned."""
         L = _lib.lib()
         _lib.require_gpu_tensor(visibility, "visibility")
         vis = visibility.reshape(-1).to(torch.uint8).contiguous()
         if vis.numel() != N:
             raise _lib.VingsError("visibility must hold N entries")
+        if max_norm is not None:
+            return self._clipped_step(L, vis, N, guard, float(max_norm))
         by_eps = {}
         for group in self.param_groups:
             if len(group["params"]) != 1:
@@ -580,3 +589,44 @@ class SparseGaussianAdam(torch.optim.Adam):
                     continue
                 check(L.vings_sparse_adam_multi(n, PP, GG, MM, VV, WW, LR, ptr(vis), b1, b2, eps,
                                                 N, stream), "vings_sparse_adam_multi")
+
+    def _clipped_step(self, L, vis, N, guard, max_norm):
+        if not max_norm >= 0.0:
+            raise _lib.VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
+        dev = vis.device
+        rows, consts = [], []
+        for group in self.param_groups:
+            if len(group["params"]) != 1:
+                raise _lib.VingsError("more than one tensor in group")
+            p = group["params"][0]
+            if p.grad is None:
+                continue
+            _lib.require_gpu_tensor(p, "param", torch.float32)
+            if p.device != dev:
+                raise _lib.VingsError("parameters and visibility must live on one device")
+            if p.grad.dtype != torch.float32:
+                raise _lib.VingsError(f"gradients must be float32 (got {p.grad.dtype})")
+            if N == 0:
+                continue
+            if p.numel() % N != 0:
+                raise _lib.VingsError("parameter size is not a multiple of N")
+            if p.numel() == 0:
+                continue
+            state = self._moments(p)
+            b1, b2 = group.get("betas", (0.9, 0.999))
+            rows.append((p, p.grad.contiguous(), state["exp_avg"], state["exp_avg_sq"]))
+            consts.append((p.numel() // N, float(group["lr"]), float(b1), float(b2), float(group["eps"])))
+        n = len(rows)
+        if n == 0:
+            return torch.zeros((), dtype=torch.float32, device=dev)
+        f = lambda k: (ctypes.c_float * n)(*[c[k] for c in consts])
+        tables = [(ctypes.c_void_p * n)(*[ptr(r[k]) for r in rows]) for k in range(4)]
+        with _lib.on_device(dev):
+            nbytes = L.vings_sparse_adam_clipped_workspace_bytes(n)
+            norm, ws = norm_and_workspace(nbytes, dev)
+            check(L.vings_sparse_adam_clipped(
+                n, *tables, (ctypes.c_int * n)(*[c[0] for c in consts]), f(1), f(2), f(3), f(4),
+                ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
+                None if guard is None else guard[0], 0 if guard is None else int(guard[1]),
+                stream_ptr(dev)), "vings_sparse_adam_clipped")
+        return norm

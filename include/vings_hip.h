@@ -282,6 +282,29 @@ int vings_grad_clip(int n_tensors, const void* const* grads_host, void* const* o
                     size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Rows of a table by id, scaled, and the gradient of the table by sorted ids.
+ *   vings_row_lookup            out[n] = scale * table[ids[n]], zeros where ids[n] is outside
+ *                               [0, n_rows)
+ *   vings_row_lookup_backward   rows[v] = scale * sum over {n : ids[n] == v} of grad[n]; rows[v]
+ *                               of an id that does not occur is zero.  Ids outside [0, n_rows)
+ *                               and ids equal to padding_id (-1: none) contribute nothing.
+ * table / grad: row-major with table_stride / grad_stride elements between rows (grad_stride 0:
+ * one row for all ids), of type VINGS_F32 / BF16 / F16; out, rows dense.  rows_type is the
+ * gradient's type or VINGS_F32.  ids int32 or int64 (id_bytes).  Sums are float32, in an order
+ * fixed by the ids alone, rounded once.  touched (may be NULL) [n_rows]: 1 for rows that some id
+ * names, else 0 -- or left as it is with keep_touched, so that several calls can mark one array.
+ * Sizes: n_ids, n_rows < 2^31 - 1, 0 < n_cols < 2^22. */
+int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, const void* table,
+                     int64_t table_stride, int type, const void* ids, int id_bytes, float scale,
+                     void* out, void* stream);
+size_t vings_row_lookup_backward_workspace_bytes(int64_t n_ids, int64_t n_cols, int type);
+int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t n_cols, const void* grad,
+                              int64_t grad_stride, int type, const void* ids, int id_bytes,
+                              int64_t padding_id, float scale, void* rows, int rows_type,
+                              uint8_t* touched, int keep_touched, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Parameter activations of get_property (gaussian_base.py:44-48,64-72):
  * opacity = sigmoid(raw), scaling = exp(raw), rotation = raw / max(|raw|, 1e-12)
  * (xyz and rgb are used as stored).  One launch for the three groups.

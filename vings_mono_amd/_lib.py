@@ -58,6 +58,12 @@ _SIGNATURES = {
     "vings_grad_norm_workspace_bytes": (_c.c_size_t, [_c.c_int, _P]),
     "vings_grad_norm": (_c.c_int, [_c.c_int] + [_P] * 3 + [_c.c_int, _P, _P, _c.c_size_t, _P]),
     "vings_grad_clip": (_c.c_int, [_c.c_int] + [_P] * 5 + [_c.c_int, _c.c_float, _P, _P, _c.c_size_t, _P]),
+    "vings_row_lookup": (_c.c_int, [_c.c_int64] * 3 + [_P, _c.c_int64, _c.c_int, _P, _c.c_int,
+                                                       _c.c_float, _P, _P]),
+    "vings_row_lookup_backward_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int64, _c.c_int]),
+    "vings_row_lookup_backward": (_c.c_int, [_c.c_int64] * 3 + [_P, _c.c_int64, _c.c_int, _P, _c.c_int,
+                                                                _c.c_int64, _c.c_float, _P, _c.c_int, _P,
+                                                                _c.c_int, _P, _c.c_size_t, _P]),
     "vings_splat_activate": (_c.c_int, [_c.c_int] + [_P] * 7),
     "vings_surfel_project_backward_finish": (_c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.c_float] +
                                              [_P] * 14 + [_c.c_int64, _c.c_int] + [_P] * 10),

@@ -30,15 +30,10 @@
 //
 // Serves the binning stage of GaussianRasterizer.forward
 // (/root/reference/scripts/gaussian/gaussian_base.py:193-203).
-#include "common.hpp"
+#include "radix_sort.hpp"
 
 namespace vings {
 
-constexpr int kSortThreads = 256;
-constexpr int kSortItems = 8;                        // keys per lane per tile
-constexpr int kSortTile = kSortThreads * kSortItems;  // 2048 keys per workgroup
-constexpr int kRadixBits = 8;
-constexpr int kRadix = 1 << kRadixBits;
 constexpr int kMaxPasses = 4;
 constexpr int kSortCap = 1024;          // composites one LDS depth sort holds (8 + 8 KB of LDS)
 
@@ -99,180 +94,6 @@ __global__ __launch_bounds__(256) void emit_keys_kernel(
         }
         tkeys[out0 + q] = tile;
         vals[out0 + q] = (uint32_t)(blockIdx.x * 256 + lo);
-    }
-}
-
-// ---------------------------------------------------------------------------
-// radix sort
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t digit_of(uint32_t k, int shift) {
-    return (k >> shift) & (kRadix - 1);
-}
-
-// Per-tile digit histogram of one pass: thist[digit][tile].
-__global__ __launch_bounds__(kSortThreads) void sort_tile_hist_kernel(
-    const uint32_t* __restrict__ keys, int64_t D, int shift, int ntiles,
-    uint32_t* __restrict__ thist, const uint32_t* __restrict__ tail) {
-    __shared__ uint32_t h[kRadix];
-    if (tail) D = min(D, (int64_t)tail[2]);
-    h[threadIdx.x] = 0;
-    __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kSortTile;
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        const int64_t i = base + r * kSortThreads + threadIdx.x;
-        if (i < D) atomicAdd(&h[digit_of(keys[i], shift)], 1u);
-    }
-    __syncthreads();
-    thist[(size_t)threadIdx.x * ntiles + blockIdx.x] = h[threadIdx.x];
-}
-
-// One 256-lane workgroup per digit: exclusive scan of that digit's row of thist (per sort
-// tile: keys with this digit in earlier tiles) and the row total into totals[digit]; the
-// scatter adds the number of keys with a smaller digit itself.  Each lane owns 8 consecutive
-// entries, so rows of up to 2048 sort tiles (4 M keys) take one round.
-constexpr int kScanItems = 8;
-__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* __restrict__ thist, int ntiles,
-                                                        uint32_t* __restrict__ totals) {
-    __shared__ uint32_t wtot[4];
-    __shared__ uint32_t carry_s;
-    const int digit = blockIdx.x;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    if (threadIdx.x == 0) carry_s = 0;
-    __syncthreads();
-    uint32_t* row = thist + (size_t)digit * ntiles;
-    for (int t0 = 0; t0 < ntiles; t0 += 256 * kScanItems) {
-        const int first = t0 + threadIdx.x * kScanItems;
-        uint32_t v[kScanItems], sum = 0;
-#pragma unroll
-        for (int k = 0; k < kScanItems; ++k) {
-            v[k] = first + k < ntiles ? row[first + k] : 0u;
-            sum += v[k];
-        }
-        const uint32_t inc = wave_scan_incl(sum);
-        if (lane == 63) wtot[w] = inc;
-        __syncthreads();
-        uint32_t run = carry_s + inc - sum;
-        for (int k = 0; k < w; ++k) run += wtot[k];
-#pragma unroll
-        for (int k = 0; k < kScanItems; ++k) {
-            if (first + k < ntiles) row[first + k] = run;
-            run += v[k];
-        }
-        __syncthreads();
-        if (threadIdx.x == 255) carry_s = run;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) totals[digit] = carry_s;
-}
-
-// Stable scatter of one tile.  Keys are held in a wave-striped arrangement
-// (item r of lane l of wave w sits at tile_base + w*512 + r*64 + l) so that
-// walking r = 0..7 visits each wave's segment in memory order.  Within a
-// round the rank of a key among equal digits is the number of lower lanes
-// holding the same digit, found with one ballot per digit bit.
-__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
-    const uint32_t* __restrict__ keys_in, const uint32_t* __restrict__ vals_in,
-    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out, int64_t D, int shift,
-    int ntiles, const uint32_t* __restrict__ thist, const uint32_t* __restrict__ totals,
-    const uint32_t* __restrict__ tail, int nbits) {
-    // nbits: significant bits of this pass's digit (the last pass of a 13-bit tile number has 5:
-    // the ballots of the bits above are all-zero and skipped)
-    __shared__ uint32_t wcount[4][kRadix];  // per-wave digit counts, then prefixes
-    if (tail) D = min(D, (int64_t)tail[2]);
-    __shared__ uint32_t gbase[kRadix];
-    __shared__ uint32_t tile_off[kRadix];
-    __shared__ uint32_t wsum4[4];
-    __shared__ uint32_t lkey[kSortTile];
-    __shared__ uint32_t lval[kSortTile];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int k = threadIdx.x; k < 4 * kRadix; k += kSortThreads) (&wcount[0][0])[k] = 0;
-    // first output slot of digit d in this tile = keys with a smaller digit anywhere
-    // (exclusive prefix of the 256 digit totals, one digit per lane) + keys with digit d in
-    // earlier tiles
-    const uint32_t tot = totals[threadIdx.x];
-    const uint32_t inc = wave_scan_incl(tot);
-    if (lane == 63) wsum4[w] = inc;
-    __syncthreads();
-    uint32_t below = inc - tot;
-    for (int k = 0; k < w; ++k) below += wsum4[k];
-    gbase[threadIdx.x] = below + thist[(size_t)threadIdx.x * ntiles + blockIdx.x];
-    __syncthreads();
-
-    const int64_t wbase = (int64_t)blockIdx.x * kSortTile + w * (kSortItems * 64);
-    uint32_t key[kSortItems];
-    uint32_t val[kSortItems];
-    uint32_t rank[kSortItems];
-    const uint64_t lt_mask = lane == 0 ? 0ull : (~0ull >> (64 - lane));
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        const int64_t i = wbase + r * 64 + lane;
-        const bool valid = i < D;
-        key[r] = valid ? keys_in[i] : ~0u;
-        val[r] = valid ? vals_in[i] : 0u;
-        const uint32_t d = digit_of(key[r], shift);
-        uint64_t peers = __ballot(valid);
-#pragma unroll
-        for (int b = 0; b < kRadixBits; ++b) {
-            if (b < nbits) {
-                const uint64_t m = __ballot((d >> b) & 1u);
-                peers &= ((d >> b) & 1u) ? m : ~m;
-            }
-        }
-        // all lanes in `peers` share digit d (invalid lanes excluded)
-        const uint32_t before = wcount[w][d];  // read before the leader updates it
-        const uint32_t below = __popcll(peers & lt_mask);
-        rank[r] = before + below;
-        __builtin_amdgcn_wave_barrier();
-        if (valid && below == 0) wcount[w][d] = before + __popcll(peers);
-        __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
-    // per digit: exclusive prefix over the 4 waves; then the digit's first slot inside the tile
-    // (exclusive prefix of the tile's digit counts over the 256 digits, one per lane)
-    {
-        const int d = threadIdx.x;
-        uint32_t run = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t c = wcount[k][d];
-            wcount[k][d] = run;
-            run += c;
-        }
-        const uint32_t inc2 = wave_scan_incl(run);
-        if (lane == 63) wsum4[w] = inc2;
-        __syncthreads();
-        uint32_t off = inc2 - run;
-        for (int k = 0; k < w; ++k) off += wsum4[k];
-        tile_off[d] = off;
-        gbase[d] -= off;   // output slot of tile position p with digit d = gbase[d] + p (mod 2^32)
-    }
-    __syncthreads();
-    // Sort the tile in LDS, then write it out in order: consecutive lanes then store to
-    // consecutive addresses inside each digit's run (a wave's store touches the few runs it
-    // spans instead of up to 64 scattered lines).
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        const int64_t i = wbase + r * 64 + lane;
-        if (i < D) {
-            const uint32_t d = digit_of(key[r], shift);
-            const uint32_t p = tile_off[d] + wcount[w][d] + rank[r];
-            lkey[p] = key[r];
-            lval[p] = val[r];
-        }
-    }
-    __syncthreads();
-    const int64_t tile_base = (int64_t)blockIdx.x * kSortTile;
-    const uint32_t n_valid = (uint32_t)max((int64_t)0, min((int64_t)kSortTile, D - tile_base));
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        const uint32_t p = r * kSortThreads + threadIdx.x;
-        if (p < n_valid) {
-            const uint32_t k = lkey[p];
-            const uint32_t dst = gbase[digit_of(k, shift)] + p;
-            keys_out[dst] = k;
-            vals_out[dst] = lval[p];
-        }
     }
 }
 
@@ -533,12 +354,6 @@ __global__ __launch_bounds__(1024) void tile_order_kernel(const uint32_t* __rest
     for (int t = threadIdx.x; t < T; t += 1024) order[atomicAdd(&cnt[cls(t)], 1u)] = (uint32_t)t;
 }
 
-static int bits_for(uint32_t span) {   // bits needed to hold values 0..span
-    int bits = 0;
-    while (bits < 32 && ((uint64_t)1 << bits) <= (uint64_t)span) ++bits;
-    return bits;
-}
-
 struct BinWorkspace {
     uint32_t* pairs;   // [2][D]: tile numbers, then splat indices (one side of the ping-pong; the
                        // other side borrows the caller's key array until the last stage fills it)
@@ -547,8 +362,6 @@ struct BinWorkspace {
     uint32_t* thist;   // [256][ntiles]
     size_t bytes;
 };
-
-static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 static BinWorkspace carve(void* ws, int64_t D) {
     BinWorkspace b;
@@ -615,14 +428,15 @@ static int bin_impl(int N, int H, int W, int64_t D, const uint32_t* tail, const 
     for (int p = 0; p < passes; ++p) {
         const int shift = p * kRadixBits;
         sort_tile_hist_kernel<<<ntiles, kSortThreads, 0, s>>>(kbuf[cur], D, shift, ntiles, b.thist,
-                                                              tail);
+                                                              tail, IdRange{});
         VINGS_LAUNCH_CHECK();
         sort_scan_kernel<<<kRadix, 256, 0, s>>>(b.thist, ntiles, b.ghist);
         VINGS_LAUNCH_CHECK();
         sort_scatter_kernel<<<ntiles, kSortThreads, 0, s>>>(kbuf[cur], vbuf[cur], kbuf[cur ^ 1],
                                                             vbuf[cur ^ 1], D, shift, ntiles,
                                                             b.thist, b.ghist, tail,
-                                                            min(kRadixBits, max(1, tile_bits - shift)));
+                                                            min(kRadixBits, max(1, tile_bits - shift)),
+                                                            IdRange{});
         VINGS_LAUNCH_CHECK();
         cur ^= 1;
     }

@@ -239,8 +239,10 @@ int vings_sparse_adam_multi(int n_groups, float* const* params_host,
 /* The same update on gradients clipped by their global norm:
  *   norm = sqrt(sum over all groups and visible rows of g^2)
  *   g' = g * min(1, max_norm / (norm + 1e-6)), then the update above on g'
- * Gradients of invisible rows count in nothing and invisible elements are not written.  A norm
- * that is infinite or NaN skips the step on the device: parameters and moments stay.  `norm`
+ * Gradients of invisible rows count in nothing; invisible rows keep their values (as above, one
+ * that shares a 16-byte quad with a visible row is written back unchanged).  A norm
+ * that is infinite or NaN skips the step on the device: parameters and moments stay.  The
+ * factors 1-b1 and 1-b2 are formed in 64 bits (vings_sparse_adam* form them in float32).  `norm`
  * (device, one float) receives the norm before clipping in every case.  Up to 64 groups, each
  * with its own b1, b2 and eps; arrays need 4-byte alignment only.  `instance_count` (may be
  * NULL) and `capacity`: as in vings_sparse_adam_multi_guarded.  The workspace holds the partial
@@ -248,8 +250,8 @@ int vings_sparse_adam_multi(int n_groups, float* const* params_host,
 size_t vings_sparse_adam_clipped_workspace_bytes(int n_groups);
 int vings_sparse_adam_clipped(int n_groups, float* const* params_host, const float* const* grads_host,
                               float* const* exp_avgs_host, float* const* exp_avg_sqs_host,
-                              const int* widths_host, const float* lrs_host, const float* b1s_host,
-                              const float* b2s_host, const float* epss_host, const uint8_t* visible,
+                              const int* widths_host, const float* lrs_host, const double* b1s_host,
+                              const double* b2s_host, const float* epss_host, const uint8_t* visible,
                               int N, float max_norm, float* norm, void* workspace,
                               size_t workspace_bytes, const uint32_t* instance_count,
                               uint32_t capacity, void* stream);
@@ -297,7 +299,8 @@ int vings_grad_clip(int n_tensors, const void* const* grads_host, void* const* o
 int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, const void* table,
                      int64_t table_stride, int type, const void* ids, int id_bytes, float scale,
                      void* out, void* stream);
-size_t vings_row_lookup_backward_workspace_bytes(int64_t n_ids, int64_t n_cols, int type);
+size_t vings_row_lookup_backward_workspace_bytes(int64_t n_ids, int64_t n_rows, int64_t n_cols,
+                                                 int type);
 int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t n_cols, const void* grad,
                               int64_t grad_stride, int type, const void* ids, int id_bytes,
                               int64_t padding_id, float scale, void* rows, int rows_type,

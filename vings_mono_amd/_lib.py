@@ -60,7 +60,7 @@ _SIGNATURES = {
     "vings_grad_clip": (_c.c_int, [_c.c_int] + [_P] * 5 + [_c.c_int, _c.c_float, _P, _P, _c.c_size_t, _P]),
     "vings_row_lookup": (_c.c_int, [_c.c_int64] * 3 + [_P, _c.c_int64, _c.c_int, _P, _c.c_int,
                                                        _c.c_float, _P, _P]),
-    "vings_row_lookup_backward_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int64, _c.c_int]),
+    "vings_row_lookup_backward_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 3 + [_c.c_int]),
     "vings_row_lookup_backward": (_c.c_int, [_c.c_int64] * 3 + [_P, _c.c_int64, _c.c_int, _P, _c.c_int,
                                                                 _c.c_int64, _c.c_float, _P, _c.c_int, _P,
                                                                 _c.c_int, _P, _c.c_size_t, _P]),
@@ -168,6 +168,8 @@ def ptr(t):
 
 
 def stream_ptr(device=None):
+    if device is not None and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -136,12 +136,17 @@ __device__ __forceinline__ uint32_t wave_scan_incl(uint32_t v) {
 }
 
 // One element of the row-masked Adam step (no bias correction, no weight decay); shared by
-// every kernel that applies it so that they agree bit for bit.
+// every kernel that applies it so that they agree bit for bit.  c1 = 1 - b1, c2 = 1 - b2.
+__device__ __forceinline__ void adam_update(float& p, float g, float& m, float& v, float lr,
+                                            float b1, float c1, float b2, float c2, float eps) {
+    m = b1 * m + c1 * g;
+    v = b2 * v + c2 * g * g;
+    p += -lr * m / (sqrtf(v) + eps);
+}
+
 __device__ __forceinline__ void adam_update(float& p, float g, float& m, float& v, float lr,
                                             float b1, float b2, float eps) {
-    m = b1 * m + (1.0f - b1) * g;
-    v = b2 * v + (1.0f - b2) * g * g;
-    p += -lr * m / (sqrtf(v) + eps);
+    adam_update(p, g, m, v, lr, b1, 1.0f - b1, b2, 1.0f - b2, eps);
 }
 
 }  // namespace vings

@@ -41,6 +41,21 @@ struct TensorTable {
     int count;
 };
 
+// The table as the waves read it: copied into LDS, an entry per lane.  Read where it stands, in
+// the kernel arguments, every step of the search would wait for its own line out of host memory.
+template <int CAP, bool OUT>
+__device__ __forceinline__ void copy_table(const TensorTable<CAP, OUT>& from, TensorTable<CAP, OUT>& to) {
+    for (int i = threadIdx.x; i <= from.count; i += blockDim.x) {
+        to.first[i] = from.first[i];
+        if (i == from.count) { to.count = from.count; break; }
+        to.in[i] = from.in[i];
+        to.n[i] = from.n[i];
+        to.type[i] = from.type[i];
+        if constexpr (OUT) { to.out[i] = from.out[i]; to.out_type[i] = from.out_type[i]; }
+    }
+    __syncthreads();
+}
+
 template <int CAP, bool OUT>
 __device__ __forceinline__ int tensor_of(const TensorTable<CAP, OUT>& T, uint32_t chunk) {
     int lo = 0, hi = T.count - 1;         // last t with first[t] <= chunk (empty tensors are left out)
@@ -120,22 +135,26 @@ __device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t o
 }
 
 // A gradient that is already short enough stays as it is: in place, nothing is read or written.
+// The chunks are taken from the last to the first: what the norm read last is still in the cache.
 __device__ __forceinline__ void range_scale(const TensorTable<kClipTensors, true>& T, uint32_t lo,
                                             uint32_t hi, int waves, float coef) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t c = lo + w;
-    if (c >= hi) return;
+    if (hi <= lo + w) return;
+    uint32_t c = hi - 1 - w;
     int t = tensor_of(T, c);
-    for (; c < hi; c += waves) {
-        while (c >= T.first[t + 1]) ++t;
-        if (coef == 1.0f && T.in[t] == T.out[t]) continue;
-        const int64_t off = (int64_t)(c - T.first[t]) * kChunk;
-        const int ty = T.type[t], ot = T.out_type[t];
-        if (ty == ELEM_F32) chunk_scale<float, float>(T.in[t], T.out[t], off, T.n[t], coef);
-        else if (ty == ELEM_BF16 && ot == ELEM_F32) chunk_scale<__bf16, float>(T.in[t], T.out[t], off, T.n[t], coef);
-        else if (ty == ELEM_BF16) chunk_scale<__bf16, __bf16>(T.in[t], T.out[t], off, T.n[t], coef);
-        else if (ot == ELEM_F32) chunk_scale<_Float16, float>(T.in[t], T.out[t], off, T.n[t], coef);
-        else chunk_scale<_Float16, _Float16>(T.in[t], T.out[t], off, T.n[t], coef);
+    for (;;) {
+        while (c < T.first[t]) --t;
+        if (coef != 1.0f || T.in[t] != T.out[t]) {
+            const int64_t off = (int64_t)(c - T.first[t]) * kChunk;
+            const int ty = T.type[t], ot = T.out_type[t];
+            if (ty == ELEM_F32) chunk_scale<float, float>(T.in[t], T.out[t], off, T.n[t], coef);
+            else if (ty == ELEM_BF16 && ot == ELEM_F32) chunk_scale<__bf16, float>(T.in[t], T.out[t], off, T.n[t], coef);
+            else if (ty == ELEM_BF16) chunk_scale<__bf16, __bf16>(T.in[t], T.out[t], off, T.n[t], coef);
+            else if (ot == ELEM_F32) chunk_scale<_Float16, float>(T.in[t], T.out[t], off, T.n[t], coef);
+            else chunk_scale<_Float16, _Float16>(T.in[t], T.out[t], off, T.n[t], coef);
+        }
+        if (c < lo + waves) break;
+        c -= waves;
     }
 }
 
@@ -146,10 +165,12 @@ __device__ __forceinline__ void block_range(uint32_t total, uint32_t& lo, uint32
 
 // One partial result per workgroup; alone, a workgroup writes the norm itself.
 template <int KIND, int CAP, bool OUT>
-__global__ __launch_bounds__(1024) void norm_partial_kernel(TensorTable<CAP, OUT> T,
+__global__ __launch_bounds__(1024) void norm_partial_kernel(TensorTable<CAP, OUT> args,
                                                             double* __restrict__ partial,
                                                             float* __restrict__ norm) {
     __shared__ double scratch[16];
+    __shared__ TensorTable<CAP, OUT> T;
+    copy_table(args, T);
     uint32_t lo, hi;
     block_range(T.first[T.count], lo, hi);
     const double v = norm_join_block<KIND>(range_norm<KIND>(T, lo, hi, blockDim.x >> 6), scratch);
@@ -168,11 +189,13 @@ __global__ __launch_bounds__(1024) void norm_final_kernel(const double* __restri
 }
 
 template <int KIND>
-__global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<kClipTensors, true> T,
+__global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<kClipTensors, true> args,
                                                          const double* __restrict__ partial,
                                                          int n_partial, float max_norm,
                                                          float* __restrict__ norm) {
     __shared__ double scratch[16];
+    __shared__ TensorTable<kClipTensors, true> T;
+    copy_table(args, T);
     const float v = norm_of_partials<KIND>(partial, n_partial, scratch);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
     uint32_t lo, hi;
@@ -182,10 +205,12 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<kClipTensor
 
 // Norm and scaling of a few chunks by one workgroup.
 template <int KIND>
-__global__ __launch_bounds__(1024) void clip_one_block_kernel(TensorTable<kClipTensors, true> T,
+__global__ __launch_bounds__(1024) void clip_one_block_kernel(TensorTable<kClipTensors, true> args,
                                                               float max_norm,
                                                               float* __restrict__ norm) {
     __shared__ double scratch[16];
+    __shared__ TensorTable<kClipTensors, true> T;
+    copy_table(args, T);
     const int waves = blockDim.x >> 6;
     const uint32_t hi = T.first[T.count];
     const double s = norm_join_block<KIND>(range_norm<KIND>(T, 0u, hi, waves), scratch);

@@ -8,10 +8,10 @@
 //
 // The gradient sums by SORTED ids, with no float atomics, so its bits do not depend on timing:
 //   1. the ids and their positions are ordered by a stable radix sort; ids that name no row sort
-//      behind the last row.  Up to 16384 ids one workgroup sorts them in LDS (registers hold the
-//      pairs between the passes) while the other workgroups of the launch clear dtable and
-//      touched, which takes longer than the sort when the table is large; more ids take the
-//      tile passes of radix_sort.hpp, 8 bits each, of which a table of 255 rows needs one
+//      behind the last row.  Up to 16384 ids workgroups sort runs of 1024 in LDS and a second
+//      launch merges the runs, every id finding its place by bisection in each of them, while
+//      further workgroups of both launches clear dtable and touched; more ids take the tile
+//      passes of radix_sort.hpp, 8 bits each
 //   2. segment kernel: the sorted positions are cut into pieces of equal length, whatever rows
 //      they belong to, so one frequent id costs no more than many rare ones.  A lane group walks
 //      a few consecutive positions, holds its columns' sum in float32 registers, and writes a
@@ -21,6 +21,10 @@
 //      first ids are equal), runs that cross workgroups leave one partial row per workgroup
 //   4. join kernel: the workgroup in whose piece such a run begins adds the partial rows of the
 //      pieces behind it, in a fixed tree
+// Few rows of few columns under many ids (per-keyframe rows) need no global order at all: a
+// workgroup sorts 1024 ids in LDS, sums their runs as in 2 and 3 and leaves one partial row per
+// row it met; a second launch adds those over the workgroups.  The gradient is then read in
+// stretches of 1024 rows instead of all over, and two launches replace seven.
 // Sums are float32 over at most 64 terms in a row, then trees; the result is scaled and rounded
 // to the gradient's type once.
 //
@@ -34,7 +38,12 @@
 
 namespace vings {
 
-constexpr int kLdsSortMax = 16384;        // ids one workgroup sorts
+constexpr int kRun = 1024;                // ids a workgroup sorts in LDS
+constexpr int kMaxRuns = 16;              // runs the merge launch takes
+constexpr int kMergeSortMax = kRun * kMaxRuns;
+constexpr int kTileIds = 1024;            // ids per workgroup of the few-rows form
+constexpr int kFewRows = 255;             // ... one 8-bit digit, the ids without a row included
+constexpr int kFewTiles = 4096;           // ... partial rows that its join adds, at most
 constexpr int kPieceMax = 2048;           // sorted positions per workgroup of the segment kernel
 
 // ---------------------------------------------------------------------------
@@ -164,101 +173,145 @@ __global__ __launch_bounds__(256) void row_clear_kernel(Fill F) {
     clear(F, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
-// Workgroup 0 sorts up to ITEMS * 1024 ids; the others clear.  The ranking is that of the tile
-// scatter (radix_sort.hpp), with sixteen waves and the pairs in registers between the passes.
-template <typename I, int ITEMS>
-__global__ __launch_bounds__(1024) void row_sort_small_kernel(const I* __restrict__ ids, int N,
-                                                              IdRange range, int bits,
-                                                              uint32_t* __restrict__ keys_out,
-                                                              uint32_t* __restrict__ vals_out,
-                                                              Fill F) {
-    __shared__ uint32_t lkey[ITEMS * 1024];
-    __shared__ uint16_t lval[ITEMS * 1024];
-    __shared__ uint16_t wcount[16][kRadix];      // a wave holds at most 64 * ITEMS <= 1024 of a digit
-    __shared__ uint32_t digit_base[kRadix];
-    __shared__ uint32_t wsum[4];
-    if (blockIdx.x > 0) {
-        clear(F, (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
-        return;
-    }
+// Stable counting sort of one digit inside a workgroup: the place of this lane's ITEMS keys
+// (item r of lane l of wave w is key number (w * ITEMS + r) * 64 + l) among the workgroup's
+// `count` valid keys.  Ranking as in the tile scatter (radix_sort.hpp).  counts: [WAVES][256],
+// base: [256], both LDS; on return base[d] is the number of keys with a smaller digit.
+template <int WAVES, int ITEMS>
+__device__ __forceinline__ void block_digit_places(const uint32_t key[ITEMS], int count, int shift, int nbits,
+                                                   uint16_t (*counts)[kRadix], uint32_t* base,
+                                                   uint32_t* wsum, uint32_t place[ITEMS]) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const uint64_t lt_mask = lane == 0 ? 0ull : (~0ull >> (64 - lane));
-    const int wbase = w * (ITEMS * 64);
-    uint32_t key[ITEMS];
-    uint16_t val[ITEMS], rank[ITEMS];
+    for (int k = threadIdx.x; k < WAVES * kRadix; k += WAVES * 64) (&counts[0][0])[k] = 0;
+    __syncthreads();
+    // which lanes hold the same digit: independent for the items, then one chain of counters
+    uint32_t below[ITEMS], peers_n[ITEMS];
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
-        const int i = wbase + r * 64 + lane;
-        key[r] = i < N ? sort_key(ids[i], range) : ~0u;
-        val[r] = (uint16_t)i;
+        const bool valid = (w * ITEMS + r) * 64 + lane < count;
+        const uint32_t d = digit_of(key[r], shift);
+        uint64_t peers = __ballot(valid);
+#pragma unroll
+        for (int b = 0; b < kRadixBits; ++b) {
+            if (b < nbits) {
+                const uint64_t m = __ballot((d >> b) & 1u);
+                peers &= ((d >> b) & 1u) ? m : ~m;
+            }
+        }
+        below[r] = __popcll(peers & lt_mask);
+        peers_n[r] = valid ? __popcll(peers) : 0u;
     }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t d = digit_of(key[r], shift);
+        const uint32_t before = counts[w][d];
+        place[r] = before + below[r];
+        __builtin_amdgcn_wave_barrier();
+        if (peers_n[r] && below[r] == 0) counts[w][d] = (uint16_t)(before + peers_n[r]);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    uint32_t run = 0, inc = 0;
+    const int d = threadIdx.x;
+    if (d < kRadix) {
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) {
+            const uint32_t c = counts[k][d];
+            counts[k][d] = (uint16_t)run;
+            run += c;
+        }
+        inc = wave_scan_incl(run);
+        if (lane == 63) wsum[w] = inc;
+    }
+    __syncthreads();
+    if (d < kRadix) {
+        uint32_t off = inc - run;
+        for (int k = 0; k < w; ++k) off += wsum[k];
+        base[d] = off;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t k = digit_of(key[r], shift);
+        place[r] += base[k] + counts[w][k];
+    }
+}
+
+// Workgroups [0, n_runs) sort 1024 ids each, the others clear.
+template <typename I>
+__global__ __launch_bounds__(1024) void row_sort_runs_kernel(const I* __restrict__ ids, int N, int n_runs,
+                                                             IdRange range, int bits,
+                                                             uint32_t* __restrict__ keys_out,
+                                                             uint32_t* __restrict__ vals_out, Fill F) {
+    __shared__ uint16_t counts[16][kRadix];
+    __shared__ uint32_t base[kRadix], wsum[4];
+    __shared__ uint32_t lkey[kRun];
+    __shared__ uint32_t lval[kRun];
+    if ((int)blockIdx.x >= n_runs) {
+        clear(F, (int64_t)(blockIdx.x - n_runs) * 1024 + threadIdx.x, (int64_t)(gridDim.x - n_runs) * 1024);
+        return;
+    }
+    const int first = blockIdx.x * kRun, t = threadIdx.x;
+    const int count = min(kRun, N - first);
+    uint32_t key[1] = {t < count ? sort_key(ids[first + t], range) : ~0u};
+    uint32_t val = (uint32_t)(first + t);
     for (int shift = 0; shift < bits; shift += kRadixBits) {
-        const int nbits = min(kRadixBits, bits - shift);
-        for (int k = threadIdx.x; k < 16 * kRadix; k += 1024) (&wcount[0][0])[k] = 0;
+        uint32_t place[1];
+        block_digit_places<16, 1>(key, count, shift, min(kRadixBits, bits - shift), counts, base, wsum, place);
+        if (t < count) { lkey[place[0]] = key[0]; lval[place[0]] = val; }
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < ITEMS; ++r) {
-            // (positions behind N are the last ones of the array and hold the largest key: they
-            // keep their place behind every id in every pass)
-            const bool valid = wbase + r * 64 + lane < N;
-            const uint32_t d = digit_of(key[r], shift);
-            uint64_t peers = __ballot(valid);
-#pragma unroll
-            for (int b = 0; b < kRadixBits; ++b) {
-                if (b < nbits) {
-                    const uint64_t m = __ballot((d >> b) & 1u);
-                    peers &= ((d >> b) & 1u) ? m : ~m;
-                }
-            }
-            const uint32_t before = wcount[w][d];
-            const uint32_t below = __popcll(peers & lt_mask);
-            rank[r] = (uint16_t)(before + below);
-            __builtin_amdgcn_wave_barrier();
-            if (valid && below == 0) wcount[w][d] = (uint16_t)(before + __popcll(peers));
-            __builtin_amdgcn_wave_barrier();
-        }
-        __syncthreads();
-        uint32_t run = 0;
-        if (threadIdx.x < kRadix) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const uint32_t c = wcount[k][threadIdx.x];
-                wcount[k][threadIdx.x] = (uint16_t)run;
-                run += c;
-            }
-            const uint32_t inc = wave_scan_incl(run);
-            if (lane == 63) wsum[w] = inc;
-            digit_base[threadIdx.x] = inc - run;
-        }
-        __syncthreads();
-        if (threadIdx.x < kRadix) {
-            uint32_t off = 0;
-            for (int k = 0; k < w; ++k) off += wsum[k];
-            digit_base[threadIdx.x] += off;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < ITEMS; ++r) {
-            if (wbase + r * 64 + lane < N) {
-                const uint32_t d = digit_of(key[r], shift);
-                const uint32_t p = digit_base[d] + wcount[w][d] + rank[r];
-                lkey[p] = key[r];
-                lval[p] = val[r];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < ITEMS; ++r) {
-            const int i = wbase + r * 64 + lane;
-            if (i < N) { key[r] = lkey[i]; val[r] = lval[i]; }
-        }
+        if (t < count) { key[0] = lkey[t]; val = lval[t]; }
         __syncthreads();
     }
-#pragma unroll
-    for (int r = 0; r < ITEMS; ++r) {
-        const int i = wbase + r * 64 + lane;
-        if (i < N) { keys_out[i] = key[r]; vals_out[i] = val[r]; }
+    if (t < count) { keys_out[first + t] = key[0]; vals_out[first + t] = val; }
+}
+
+// Merges up to kMaxRuns sorted runs: the place of an id is its place in its own run plus, for
+// every earlier run, the ids there that are not larger, and for every later one those that are
+// smaller.  All keys sit in LDS; four bisections of a lane run side by side.
+constexpr int kMergeThreads = 256;
+__global__ __launch_bounds__(kMergeThreads) void row_merge_runs_kernel(
+    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int N, int n_runs, int n_merge,
+    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out, Fill F) {
+    __shared__ __align__(16) uint32_t lkey[kMergeSortMax];
+    if ((int)blockIdx.x >= n_merge) {
+        clear(F, (int64_t)(blockIdx.x - n_merge) * kMergeThreads + threadIdx.x,
+              (int64_t)(gridDim.x - n_merge) * kMergeThreads);
+        return;
     }
+    for (int i = 4 * threadIdx.x; i < n_runs * kRun; i += 4 * kMergeThreads) {
+        if (i + 4 <= N) {
+            *reinterpret_cast<uint4*>(lkey + i) = *reinterpret_cast<const uint4*>(keys + i);
+        } else {
+            for (int k = i; k < i + 4; ++k) lkey[k] = k < N ? keys[k] : ~0u;
+        }
+    }
+    __syncthreads();
+    const int e = blockIdx.x * kMergeThreads + threadIdx.x;
+    if (e >= N) return;
+    const uint32_t key = lkey[e];
+    const int own = e / kRun;
+    uint32_t place = (uint32_t)(e - own * kRun);
+    for (int r0 = 0; r0 < n_runs; r0 += 4) {
+        uint32_t pos[4] = {0, 0, 0, 0}, limit[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) limit[u] = key + (r0 + u < own ? 1u : 0u);
+#pragma unroll
+        for (int step = kRun / 2; step > 0; step >>= 1)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int r = min(r0 + u, n_runs - 1);
+                if (lkey[r * kRun + pos[u] + step - 1] < limit[u]) pos[u] += step;
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u;
+            if (r < n_runs && r != own) place += pos[u] + (lkey[r * kRun + pos[u]] < limit[u] ? 1u : 0u);
+        }
+    }
+    keys_out[place] = key;
+    vals_out[place] = vals[e];
 }
 
 // ---------------------------------------------------------------------------
@@ -277,70 +330,45 @@ struct Segments {
     float* partial;           // [piece][2][D]: {run from an earlier piece, run into the next}
 };
 
-template <int V>
-__device__ __forceinline__ void store_partial(float* __restrict__ p, const float f[V]) {
-    if constexpr (V == 8) store_cols<float, 8>(p, f);
-    else store_cols<float, V>(p, f);
-}
+// Sums of the runs of equal keys among a workgroup's `len` sorted positions.  skey[1 .. len]: the
+// keys, skey[0] and skey[len + 1] those before and behind them (kNoKey where there are none);
+// spos: the gradient rows.  Calls write(row, sum) for runs that lie inside, head(sum) for the one
+// that began before, tail(sum, all) for the one that goes on behind (all: and began before), and
+// begin(row) where a run begins; every call comes from the lanes that hold the sum's columns.
+constexpr uint32_t kNoKey = ~0u;                     // rows < 2^31
+template <int V> struct RunShared {
+    float val[256 * V];                              // open sums, lane-contiguous per component
+    uint8_t open[256];                               // a group's open sum reaches the left edge
+};
 
-template <typename T, typename O, int V>
-__global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* __restrict__ grad,
-                                                          O* __restrict__ out) {
+template <typename T, int V, typename W, typename H, typename L, typename B>
+__device__ __forceinline__ void sum_runs(const Segments& S, const T* __restrict__ grad, const uint32_t* skey,
+                                         const uint32_t* spos, int len, bool col_ok, int64_t c,
+                                         RunShared<V>& sh, W write, H write_head, L write_tail, B begin) {
     typedef typename VecOf<T, V>::type vec;
-    __shared__ uint32_t skey[kPieceMax + 2];          // with the key before and behind the piece
-    __shared__ uint32_t spos[kPieceMax];
-    __shared__ float sval[256 * V];                   // open sums, lane-contiguous per component
-    __shared__ uint8_t sopen[256];                    // group's open sum reaches its left edge
-    constexpr uint32_t kNone = ~0u;                   // no such key: rows < 2^31
     const int lanes = 1 << S.lg, n_groups = 256 >> S.lg;
     const int g = threadIdx.x >> S.lg;
-    const int64_t j = (int64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
-    const bool col_ok = j * V < S.D;
-    const int64_t c = col_ok ? vec_col<V>(j, S.D) : 0;
-    const int piece = n_groups * S.per_group;
-    const int64_t base = (int64_t)blockIdx.x * piece;
-    const int len = (int)min((int64_t)piece, (int64_t)S.N - base);
-    for (int i = threadIdx.x; i < len + 2; i += 256) {
-        const int64_t q = base + i - 1;
-        skey[i] = q >= 0 && q < S.N ? S.keys[q] : kNone;
-    }
-    for (int i = threadIdx.x; i < len; i += 256) spos[i] = S.pos[base + i];
-    __syncthreads();
-
     const int first = min(g * S.per_group, len), last = min(first + S.per_group, len);
     float acc[V], head[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] = head[k] = 0.f;
-    uint32_t cur = kNone;
+    uint32_t cur = kNoKey, head_key = kNoKey;
     bool from_left = false;            // the run being summed began before this group's positions
     bool has_head = false, has_tail = false;
-    uint32_t head_key = kNone;
-
-    auto write_row = [&](uint32_t row, const float f[V]) {
-        if (row >= S.rows || !col_ok) return;
-        float o[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = f[k] * S.scale;
-        store_cols<O, V>(out + (int64_t)row * S.D + c, o);
-    };
     auto close_run = [&] {
         if (from_left) {
             has_head = true; head_key = cur;
 #pragma unroll
             for (int k = 0; k < V; ++k) head[k] = acc[k];
-        } else {
-            write_row(cur, acc);
+        } else if (cur < S.rows && col_ok) {
+            write(cur, acc);
         }
     };
-
     if (first < last) {
         cur = skey[first + 1];
         from_left = skey[first] == cur;
-        auto begin_row = [&](uint32_t row) {
-            if (S.touched && row < S.rows && j == 0) S.touched[row] = 1;
-        };
-        if (!from_left) begin_row(cur);
-        constexpr int U = 4;
+        if (!from_left && cur < S.rows) begin(cur);
+        constexpr int U = 8;
         for (int i0 = first; i0 < last; i0 += U) {
             vec v[U];
 #pragma unroll
@@ -357,7 +385,7 @@ __global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* _
                 if (k_i != cur) {
                     close_run();
                     cur = k_i; from_left = false;
-                    begin_row(cur);
+                    if (cur < S.rows) begin(cur);
 #pragma unroll
                     for (int k = 0; k < V; ++k) acc[k] = 0.f;
                 }
@@ -377,42 +405,78 @@ __global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* _
     bool open = has_tail && from_left;
     const int l = threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < V; ++k) sval[k * 256 + l] = acc[k];
-    sopen[l] = open;
-    __syncthreads();
+    for (int k = 0; k < V; ++k) sh.val[k * 256 + l] = acc[k];
+    sh.open[l] = open;
     for (int s = 1; s < n_groups; s <<= 1) {
         const int q = l - (s << S.lg);
         const bool add = open && q >= 0;
+        if (!__syncthreads_or(add)) break;
         float t[V];
         bool o = open;
         if (add) {
-            o = sopen[q];
+            o = sh.open[q];
 #pragma unroll
-            for (int k = 0; k < V; ++k) t[k] = sval[k * 256 + q];
+            for (int k = 0; k < V; ++k) t[k] = sh.val[k * 256 + q];
         }
         __syncthreads();
         if (add) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) sval[k * 256 + l] = acc[k] = t[k] + acc[k];
-            sopen[l] = open = o;
+            for (int k = 0; k < V; ++k) sh.val[k * 256 + l] = acc[k] = t[k] + acc[k];
+            sh.open[l] = open = o;
         }
-        __syncthreads();
     }
+    __syncthreads();
     // (open now: the run fills everything from the workgroup's left edge to this group's end)
     if (has_head) {
         bool before_piece = true;
         if (g > 0) {
             const int q = l - lanes;
-            before_piece = sopen[q];
+            before_piece = sh.open[q];
 #pragma unroll
-            for (int k = 0; k < V; ++k) head[k] += sval[k * 256 + q];
+            for (int k = 0; k < V; ++k) head[k] += sh.val[k * 256 + q];
         }
-        if (!before_piece) write_row(head_key, head);
-        else if (col_ok && head_key < S.rows)
-            store_partial<V>(S.partial + ((int64_t)blockIdx.x * 2) * S.D + c, head);
+        if (head_key < S.rows && col_ok) {
+            if (before_piece) write_head(head); else write(head_key, head);
+        }
     }
-    if (has_tail && last == len && cur < S.rows && col_ok)
-        store_partial<V>(S.partial + ((int64_t)blockIdx.x * 2 + (open ? 0 : 1)) * S.D + c, acc);
+    if (has_tail && last == len && cur < S.rows && col_ok) write_tail(acc, open);
+}
+
+template <typename O, int V>
+__device__ __forceinline__ void write_scaled(O* __restrict__ p, const float f[V], float scale) {
+    float o[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = f[k] * scale;
+    store_cols<O, V>(p, o);
+}
+
+template <typename T, typename O, int V>
+__global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* __restrict__ grad,
+                                                          O* __restrict__ out) {
+    extern __shared__ uint32_t smem[];                // (the usual piece takes a few hundred bytes)
+    __shared__ RunShared<V> sh;
+    const int lanes = 1 << S.lg;
+    const int64_t j = (int64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+    const bool col_ok = j * V < S.D;
+    const int64_t c = col_ok ? vec_col<V>(j, S.D) : 0;
+    const int piece = (256 >> S.lg) * S.per_group;
+    uint32_t* skey = smem;                            // with the keys before and behind the piece
+    uint32_t* spos = smem + piece + 2;
+    const int64_t base = (int64_t)blockIdx.x * piece;
+    const int len = (int)min((int64_t)piece, (int64_t)S.N - base);
+    for (int i = threadIdx.x; i < len + 2; i += 256) {
+        const int64_t q = base + i - 1;
+        skey[i] = q >= 0 && q < S.N ? S.keys[q] : kNoKey;
+    }
+    for (int i = threadIdx.x; i < len; i += 256) spos[i] = S.pos[base + i];
+    __syncthreads();
+    float* partial = S.partial + (int64_t)blockIdx.x * 2 * S.D + c;
+    sum_runs<T, V>(
+        S, grad, skey, spos, len, col_ok, c, sh,
+        [&](uint32_t row, const float* f) { write_scaled<O, V>(out + (int64_t)row * S.D + c, f, S.scale); },
+        [&](const float* f) { store_cols<float, V>(partial, f); },
+        [&](const float* f, bool all) { store_cols<float, V>(partial + (all ? 0 : S.D), f); },
+        [&](uint32_t row) { if (S.touched && j == 0) S.touched[row] = 1; });
 }
 
 // One workgroup per piece and column segment; those in whose piece no run begins that goes on
@@ -465,20 +529,132 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
             }
         }
     }
-    if (g == 0 && col_ok) {
+    if (g == 0 && col_ok) write_scaled<O, V>(out + (int64_t)k * S.D + c, acc, S.scale);
+}
+
+// ---------------------------------------------------------------------------
+// gradient, few rows: at most 255 rows of at most 16 vectors
+// ---------------------------------------------------------------------------
+// The workgroup's own stable order of its 1024 ids, then their runs.  With one workgroup the sums
+// are the rows themselves; otherwise row r of tile t goes to partial[r][t], met[r][t] says
+// whether the tile has it.
+template <typename T, typename O, typename I, int V>
+__global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __restrict__ grad,
+                                                       const I* __restrict__ ids, IdRange range, int bits,
+                                                       O* __restrict__ out, uint8_t* __restrict__ met,
+                                                       int keep_touched) {
+    __shared__ uint16_t counts[4][kRadix];
+    __shared__ uint32_t base[kRadix + 1], wsum[4];
+    __shared__ uint32_t skey[kTileIds + 2];
+    __shared__ uint32_t spos[kTileIds];
+    __shared__ RunShared<V> sh;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * kTileIds;
+    const int len = (int)min((int64_t)kTileIds, (int64_t)S.N - first);
+    uint32_t key[4], place[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] *= S.scale;
-        store_cols<O, V>(out + (int64_t)k * S.D + c, acc);
+    for (int r = 0; r < 4; ++r) {
+        const int i = (w * 4 + r) * 64 + lane;
+        key[r] = i < len ? sort_key(ids[first + i], range) : ~0u;
     }
+    block_digit_places<4, 4>(key, len, 0, bits, counts, base, wsum, place);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int i = (w * 4 + r) * 64 + lane;
+        if (i < len) { skey[place[r] + 1] = key[r]; spos[place[r]] = (uint32_t)i; }
+    }
+    if (threadIdx.x == 0) { skey[0] = skey[len + 1] = kNoKey; base[kRadix] = (uint32_t)len; }
+    __syncthreads();
+    const bool alone = gridDim.x == 1;
+    const int64_t tiles = gridDim.x;
+    for (uint32_t r = threadIdx.x; r < S.rows; r += 256) {
+        const uint8_t any = base[r + 1] > base[r];
+        if (!alone) met[r * tiles + blockIdx.x] = any;
+        else if (S.touched && (any || !keep_touched)) S.touched[r] = any;
+    }
+    const int lanes = 1 << S.lg;
+    const int64_t j = threadIdx.x & (lanes - 1);
+    const bool col_ok = j * V < S.D;
+    const int64_t c = col_ok ? vec_col<V>(j, S.D) : 0;
+    if (alone && col_ok) {
+        const float zero[V] = {};
+        for (uint32_t r = threadIdx.x >> S.lg; r < S.rows; r += 256 >> S.lg)
+            if (base[r + 1] == base[r]) store_cols<O, V>(out + (int64_t)r * S.D + c, zero);
+    }
+    sum_runs<T, V>(
+        S, grad + first * S.ld, skey, spos, len, col_ok, c, sh,
+        [&](uint32_t row, const float* f) {
+            if (alone) write_scaled<O, V>(out + (int64_t)row * S.D + c, f, S.scale);
+            else store_cols<float, V>(S.partial + (row * tiles + blockIdx.x) * S.D + c, f);
+        },
+        [](const float*) {}, [](const float*, bool) {}, [](uint32_t) {});
+}
+
+// One workgroup per row: its partial rows over the tiles, in a fixed tree.
+template <typename O, int V>
+__global__ __launch_bounds__(256) void row_tile_join_kernel(Segments S, const uint8_t* __restrict__ met, int tiles,
+                                                            O* __restrict__ out, int keep_touched) {
+    __shared__ float sval[256 * V];
+    const int lanes = 1 << S.lg, n_groups = 256 >> S.lg;
+    const int g = threadIdx.x >> S.lg;
+    const int64_t row = blockIdx.x, j = threadIdx.x & (lanes - 1);
+    const bool col_ok = j * V < S.D;
+    const int64_t c = col_ok ? vec_col<V>(j, S.D) : 0;
+    const float* __restrict__ part = S.partial + row * tiles * S.D + c;
+    const uint8_t* __restrict__ has = met + row * tiles;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    int any = 0;
+    constexpr int U = 4;
+    for (int t0 = g; t0 < tiles; t0 += U * n_groups) {
+        bool in[U];
+        float f[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + u * n_groups;
+            in[u] = t < tiles && has[t];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (in[u] && col_ok) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[u][i] = part[(int64_t)(t0 + u * n_groups) * S.D + i];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (in[u] && col_ok) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] += f[u][i];
+            }
+            any |= in[u];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sval[i * 256 + threadIdx.x] = acc[i];
+    any = __syncthreads_or(any);
+    for (int s = n_groups >> 1; s > 0; s >>= 1) {
+        if (g < s) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                acc[i] += sval[i * 256 + threadIdx.x + (s << S.lg)];
+                sval[i * 256 + threadIdx.x] = acc[i];
+            }
+        }
+        __syncthreads();
+    }
+    if (g == 0 && col_ok) write_scaled<O, V>(out + row * S.D + c, acc, S.scale);
+    if (threadIdx.x == 0 && S.touched && (any || !keep_touched)) S.touched[row] = any != 0;
 }
 
 namespace {
 
 int ceil_log2(int64_t x) { int l = 0; while (((int64_t)1 << l) < x) ++l; return l; }
 
-// How the gradient is cut up: by the number of ids, columns and the vector width alone.
-struct SegmentPlan { int vec, lg, per_group, pieces, segments; };
-SegmentPlan plan_segments(int64_t N, int64_t D, int type) {
+// How the gradient is cut up: by the numbers of ids, rows and columns and the vector width alone.
+struct SegmentPlan { bool few; int vec, lg, per_group, pieces, segments; };
+SegmentPlan plan_segments(int64_t N, int64_t rows, int64_t D, int type) {
     SegmentPlan p;
     const int full = type == ELEM_F32 ? 4 : 8;
     p.vec = D >= full ? full : 1;
@@ -486,12 +662,22 @@ SegmentPlan plan_segments(int64_t N, int64_t D, int type) {
     p.lg = vectors >= 64 ? 6 : ceil_log2(vectors);
     p.segments = (int)((vectors + (1 << p.lg) - 1) >> p.lg);
     const int groups = 256 >> p.lg;
+    // few rows: one digit, a lane group of the tile sums at most 64 positions, the partial rows
+    // stay below a quarter of the gradient
+    p.few = rows <= kFewRows && vectors <= 16 && N <= (int64_t)kFewTiles * kTileIds;
+    if (p.few) {
+        p.per_group = (int)((std::min<int64_t>(N, kTileIds) + groups - 1) / groups);
+        p.pieces = (int)((N + kTileIds - 1) / kTileIds);
+        return p;
+    }
     // about 2048 workgroups (eight per CU) where there are enough ids; 4 positions at least (the
     // loads a lane keeps in flight), 64 at most (what one float32 sum may run over)
-    int64_t per = N * p.segments / ((int64_t)groups * 2048);
+    const int64_t per = N * p.segments / ((int64_t)groups * 2048);
     p.per_group = 4;
     while (p.per_group < per && p.per_group < 64 && groups * p.per_group < kPieceMax) p.per_group *= 2;
-    // (a piece of few groups still takes a few dozen ids: fewer partial rows to join)
+    // (a few ids more per group spare the join)
+    while (p.per_group < 16 && groups * p.per_group < N && groups * 16 >= N &&
+           groups * p.per_group < kPieceMax) p.per_group *= 2;
     const int piece = groups * p.per_group;
     p.pieces = (int)((N + piece - 1) / piece);
     return p;
@@ -500,36 +686,56 @@ SegmentPlan plan_segments(int64_t N, int64_t D, int type) {
 struct GradWorkspace {
     uint32_t *key[2], *val[2], *thist, *totals;
     float* partial;
+    uint8_t* met;
     size_t bytes;
 };
-GradWorkspace carve_grad(void* ws, int64_t N, int64_t D, int type) {
+GradWorkspace carve_grad(void* ws, const SegmentPlan& s, int64_t N, int64_t rows, int64_t D) {
     GradWorkspace w;
     char* p = (char*)ws;
     size_t off = 0;
     auto take = [&](size_t bytes) { char* q = p + off; off += align256(bytes); return q; };
-    const bool tiles = N > kLdsSortMax;
+    const bool tiles = !s.few && N > kMergeSortMax;
     for (int i = 0; i < 2; ++i) {
-        const bool need = i == 0 || tiles;
+        const bool need = !s.few && (i == 0 || N > kRun);
         w.key[i] = (uint32_t*)take(need ? 4 * (size_t)N : 0);
         w.val[i] = (uint32_t*)take(need ? 4 * (size_t)N : 0);
     }
     const size_t ntiles = ((size_t)N + kSortTile - 1) / kSortTile;
     w.thist = (uint32_t*)take(tiles ? 4 * kRadix * ntiles : 0);
     w.totals = (uint32_t*)take(tiles ? 4 * kRadix : 0);
-    const SegmentPlan s = plan_segments(N, D, type);
-    w.partial = (float*)take(s.pieces > 1 ? sizeof(float) * 2 * (size_t)s.pieces * D : 0);
+    const size_t slots = s.pieces <= 1 ? 0 : (size_t)s.pieces * (s.few ? (size_t)rows : 2);
+    w.partial = (float*)take(sizeof(float) * slots * D);
+    w.met = (uint8_t*)take(s.few ? slots : 0);
     w.bytes = off;
     return w;
 }
 
+// Leaves the sorted pairs in key[*at], val[*at].
 template <typename I>
-int sort_small(const I* ids, int N, IdRange range, int bits, const GradWorkspace& w, const Fill& F,
-               int clear_blocks, hipStream_t s) {
-    const int grid = 1 + clear_blocks;
-    if (N <= 1024) row_sort_small_kernel<I, 1><<<grid, 1024, 0, s>>>(ids, N, range, bits, w.key[0], w.val[0], F);
-    else if (N <= 4096) row_sort_small_kernel<I, 4><<<grid, 1024, 0, s>>>(ids, N, range, bits, w.key[0], w.val[0], F);
-    else row_sort_small_kernel<I, 16><<<grid, 1024, 0, s>>>(ids, N, range, bits, w.key[0], w.val[0], F);
+int sort_runs(const I* ids, int N, IdRange range, int bits, const GradWorkspace& w, const Fill& F, int* at,
+              hipStream_t s) {
+    const int runs = cdiv(N, kRun);
+    // clearing in 64 KB per workgroup, four per CU at most; three quarters beside the first
+    // launch, which leaves more of every CU free
+    auto blocks = [](const Fill& f) {
+        return (int)std::min<int64_t>(1024, (f.bytes + f.n_touched + 65535) / 65536);
+    };
+    Fill A = F, B = F;
+    if (runs > 1) {
+        A.bytes = (F.bytes / 4 * 3) & ~(int64_t)15;
+        A.n_touched = 0;
+        B.rows = (char*)F.rows + A.bytes;
+        B.bytes = F.bytes - A.bytes;
+    }
+    row_sort_runs_kernel<I><<<runs + blocks(A), 1024, 0, s>>>(ids, N, runs, range, bits, w.key[0], w.val[0], A);
     VINGS_LAUNCH_CHECK();
+    *at = 0;
+    if (runs == 1) return VINGS_OK;
+    const int merge = cdiv(N, kMergeThreads);
+    row_merge_runs_kernel<<<merge + blocks(B), kMergeThreads, 0, s>>>(w.key[0], w.val[0], N, runs, merge,
+                                                                      w.key[1], w.val[1], B);
+    VINGS_LAUNCH_CHECK();
+    *at = 1;
     return VINGS_OK;
 }
 
@@ -565,13 +771,37 @@ int sort_tiles(const I* ids, int64_t N, IdRange range, int bits, const GradWorks
 
 template <typename T, typename O, int V>
 int segment_launches(const Segments& S, const SegmentPlan& p, const void* grad, void* out, hipStream_t s) {
-    row_segment_kernel<T, O, V><<<dim3(p.pieces, p.segments), 256, 0, s>>>(S, (const T*)grad, (O*)out);
+    row_segment_kernel<T, O, V><<<dim3(p.pieces, p.segments), 256, 4 * (2 * ((256 >> p.lg) * p.per_group) + 2), s>>>(S, (const T*)grad, (O*)out);
     VINGS_LAUNCH_CHECK();
     if (p.pieces > 1) {
         row_join_kernel<O, V><<<dim3(p.pieces - 1, p.segments), 256, 0, s>>>(S, (O*)out, p.pieces);
         VINGS_LAUNCH_CHECK();
     }
     return VINGS_OK;
+}
+
+template <typename T, typename O, typename I, int V>
+int few_launches(const Segments& S, const SegmentPlan& p, const GradWorkspace& w, const void* grad, const void* ids,
+                 IdRange range, int bits, void* out, int keep_touched, hipStream_t s) {
+    row_tile_kernel<T, O, I, V><<<p.pieces, 256, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out, w.met,
+                                                         keep_touched);
+    VINGS_LAUNCH_CHECK();
+    if (p.pieces > 1) {
+        row_tile_join_kernel<O, V><<<(int)S.rows, 256, 0, s>>>(S, w.met, p.pieces, (O*)out, keep_touched);
+        VINGS_LAUNCH_CHECK();
+    }
+    return VINGS_OK;
+}
+
+template <typename T, typename O>
+int few_by_kind(const Segments& S, const SegmentPlan& p, const GradWorkspace& w, const void* grad, const void* ids,
+                int id_bytes, IdRange range, int bits, void* out, int keep, hipStream_t s) {
+    constexpr int V = Elem<T>::kVec;
+    if (id_bytes == 8)
+        return p.vec == 1 ? few_launches<T, O, int64_t, 1>(S, p, w, grad, ids, range, bits, out, keep, s)
+                          : few_launches<T, O, int64_t, V>(S, p, w, grad, ids, range, bits, out, keep, s);
+    return p.vec == 1 ? few_launches<T, O, int32_t, 1>(S, p, w, grad, ids, range, bits, out, keep, s)
+                      : few_launches<T, O, int32_t, V>(S, p, w, grad, ids, range, bits, out, keep, s);
 }
 
 template <typename T, typename O>
@@ -645,9 +875,11 @@ extern "C" int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, c
     return lookup_by_id<_Float16>(id_bytes, n_ids, n_cols, table, table_stride, ids, range, scale, out, s);
 }
 
-extern "C" size_t vings_row_lookup_backward_workspace_bytes(int64_t n_ids, int64_t n_cols, int type) {
-    if (n_ids <= 0 || n_cols <= 0 || n_ids >= ((int64_t)1 << 31) || !elem_known(type)) return 0;
-    return carve_grad(nullptr, n_ids, n_cols, type).bytes;
+extern "C" size_t vings_row_lookup_backward_workspace_bytes(int64_t n_ids, int64_t n_rows, int64_t n_cols,
+                                                            int type) {
+    const int64_t top = (int64_t)1 << 31;
+    if (n_ids <= 0 || n_rows <= 0 || n_cols <= 0 || n_ids >= top || n_cols >= (1 << 22) || !elem_known(type)) return 0;
+    return carve_grad(nullptr, plan_segments(n_ids, n_rows, n_cols, type), n_ids, n_rows, n_cols).bytes;
 }
 
 extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t n_cols,
@@ -664,31 +896,44 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
     VINGS_REQUIRE(((uintptr_t)rows & (elem_bytes(rows_type) - 1)) == 0, "element alignment");
     hipStream_t s = (hipStream_t)stream;
     const Fill F{rows, n_rows * n_cols * elem_bytes(rows_type), touched, touched && !keep_touched ? n_rows : 0};
-    // clearing: 64 KB per workgroup, eight workgroups per CU at most
-    const int64_t per = 65536;
-    int clear_blocks = (int)std::min<int64_t>(2048, (F.bytes + F.n_touched + per - 1) / per);
+    // clearing in a launch of its own: 64 KB per workgroup, eight workgroups per CU at most
+    const int clear_blocks = (int)std::min<int64_t>(2048, (F.bytes + F.n_touched + 65535) / 65536);
     ProfScope prof(PROF_AUX, s);
     if (n_ids == 0) {
         row_clear_kernel<<<clear_blocks, 256, 0, s>>>(F);
         VINGS_LAUNCH_CHECK();
         return VINGS_OK;
     }
-    VINGS_REQUIRE(grad && ids && workspace, "null pointer");
+    VINGS_REQUIRE(grad && ids, "null pointer");
     VINGS_REQUIRE(grad_stride >= 0, "sizes");
     VINGS_REQUIRE(((uintptr_t)grad & (elem_bytes(type) - 1)) == 0 && ((uintptr_t)ids & (id_bytes - 1)) == 0,
                   "element alignment");
     VINGS_REQUIRE(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
-    const GradWorkspace w = carve_grad(workspace, n_ids, n_cols, type);
+    const SegmentPlan p = plan_segments(n_ids, n_rows, n_cols, type);
+    const GradWorkspace w = carve_grad(workspace, p, n_ids, n_rows, n_cols);
     if (workspace_bytes < w.bytes) {
         set_error("row gradient workspace too small: %zu < %zu", workspace_bytes, w.bytes);
         return VINGS_ERR_CAPACITY;
     }
+    VINGS_REQUIRE(workspace || w.bytes == 0, "null pointer");
     const IdRange range{(uint32_t)n_rows, padding_id};
     const int bits = std::max(1, bits_for((uint32_t)n_rows));
+    Segments S{nullptr, nullptr, (int)n_ids, (uint32_t)n_rows, n_cols, grad_stride, p.lg, p.per_group, scale, touched,
+               w.partial};
+    if (p.few) {
+        if (type == ELEM_F32) return few_by_kind<float, float>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s);
+        if (type == ELEM_BF16)
+            return rows_type == ELEM_F32
+                ? few_by_kind<__bf16, float>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s)
+                : few_by_kind<__bf16, __bf16>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s);
+        return rows_type == ELEM_F32
+            ? few_by_kind<_Float16, float>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s)
+            : few_by_kind<_Float16, _Float16>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s);
+    }
     int at = 0, rs;
-    if (n_ids <= kLdsSortMax) {
-        rs = id_bytes == 8 ? sort_small((const int64_t*)ids, (int)n_ids, range, bits, w, F, clear_blocks, s)
-                           : sort_small((const int32_t*)ids, (int)n_ids, range, bits, w, F, clear_blocks, s);
+    if (n_ids <= kMergeSortMax) {
+        rs = id_bytes == 8 ? sort_runs((const int64_t*)ids, (int)n_ids, range, bits, w, F, &at, s)
+                           : sort_runs((const int32_t*)ids, (int)n_ids, range, bits, w, F, &at, s);
     } else {
         row_clear_kernel<<<clear_blocks, 256, 0, s>>>(F);
         VINGS_LAUNCH_CHECK();
@@ -696,9 +941,9 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
                            : sort_tiles((const int32_t*)ids, n_ids, range, bits, w, &at, s);
     }
     if (rs != VINGS_OK) return rs;
-    const SegmentPlan p = plan_segments(n_ids, n_cols, type);
-    const Segments S{w.key[at], w.val[at], (int)n_ids, (uint32_t)n_rows, n_cols, grad_stride, p.lg,
-                     p.per_group, scale, touched, w.partial};
+    VINGS_REQUIRE((256 >> p.lg) * p.per_group <= kPieceMax, "piece");
+    S.keys = w.key[at];
+    S.pos = w.val[at];
     if (type == ELEM_F32) return segment_by_width<float, float>(S, p, grad, rows, s);
     if (type == ELEM_BF16)
         return rows_type == ELEM_F32 ? segment_by_width<__bf16, float>(S, p, grad, rows, s)

@@ -107,47 +107,55 @@ __global__ __launch_bounds__(256) void sparse_adam_multi_kernel(AdamGroups G,
 // element 4 B of gradient twice and 24 B of parameter and moments, where clipping first moves
 // another 8 B and a launch.  HBM-bound.
 // ---------------------------------------------------------------------------
-constexpr int kNormBlocks = 512;       // partial results per launch
+constexpr int kNormBlocks = 1024;      // partial results per launch
 constexpr int kStepBlocks = 2048;      // eight workgroups per CU share the reading of the partials
 constexpr int kMaxClipGroups = 64;
 
 typedef Elem<float>::vec quad_t;       // 16-byte access at any 4-byte boundary
 
-// Which of the four elements from e0 lie in visible rows (elements at or behind `total` do not).
+// Which of the four elements from e0 (a multiple of 4) lie in visible rows; elements at or behind
+// `total` do not.  Four elements touch four rows of one float, else two at most.
 template <typename I>
 __device__ __forceinline__ int visible_quad(const uint8_t* __restrict__ visible, I e0, I total, int M) {
-    if (M >= 4 && e0 + 4 <= total) {
-        const I r = M == 4 ? e0 >> 2 : e0 / (I)M;
-        const I left = (r + 1) * (I)M - e0;           // elements of row r from e0 on
-        const int a = visible[r] ? 0xF : 0;
-        if (left >= 4) return a;
-        const int low = (1 << (int)left) - 1;
-        return (a & low) | (visible[r + 1] ? 0xF & ~low : 0);
-    }
-    int m = 0;
+    const int n = total - e0 >= 4 ? 4 : (int)(total - e0);
+    if (M == 1) {
+        int m = 0;
+        if (n == 4) {
+            typedef uint8_t u8x4 __attribute__((ext_vector_type(4), aligned(1)));
+            const u8x4 v = *reinterpret_cast<const u8x4*>(visible + e0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (e0 + k < total && visible[row_of(e0 + k, M)]) m |= 1 << k;
-    return m;
+            for (int k = 0; k < 4; ++k) m |= v[k] ? 1 << k : 0;
+        } else {
+            for (int k = 0; k < n; ++k) m |= visible[e0 + k] ? 1 << k : 0;
+        }
+        return m;
+    }
+    const I r = row_of<I>(e0, M);
+    const I left = (r + 1) * (I)M - e0;               // elements of row r from e0 on
+    const int low = left >= 4 ? 0xF : (1 << (int)left) - 1;
+    int m = visible[r] ? low : 0;
+    if (left < (I)n && visible[r + 1]) m |= 0xF & ~low;
+    return m & ((1 << n) - 1);
 }
 
-// Calls f(group, first element, length of the group's arrays, visibility bits) for every quad
-// with a visible element that this workgroup serves.
-template <typename F>
-__device__ __forceinline__ void for_visible_quads(const AdamGroups& G, const uint8_t* __restrict__ visible,
-                                                  int N, F f) {
-    int g = 0;
-    for (int b = blockIdx.x; b < G.first_block[G.n]; b += gridDim.x) {
-        while (b >= G.first_block[g + 1]) ++g;
-        const int M = G.width[g];
-        const int64_t total = (int64_t)N * M;
-        const int64_t e0 = ((int64_t)(b - G.first_block[g]) * 256 + threadIdx.x) * 4;
-        if (e0 >= total) continue;
-        // (32-bit row arithmetic wherever the array allows it: a 64-bit division is a subroutine)
-        const int m = total <= 0x7FFFFFFFll ? visible_quad<uint32_t>(visible, (uint32_t)e0, (uint32_t)total, M)
-                                            : visible_quad<int64_t>(visible, e0, total, M);
-        if (m) f(g, e0, total, m);
-    }
+// A quad of one group's arrays: where it starts, and which of its elements are stepped.
+struct Quad { int g, mask; int64_t e0, total; };
+
+// The quad of this lane in block b of the launch's quads (256 consecutive ones of one group);
+// mask 0 behind the end.  `g` is a hint: a group that does not lie behind b's.
+__device__ __forceinline__ Quad quad_of(const AdamGroups& G, const uint8_t* __restrict__ visible, int N,
+                                        int64_t b, int g) {
+    Quad q{g, 0, 0, 0};
+    if (b >= G.first_block[G.n]) return q;
+    while (b >= G.first_block[q.g + 1]) ++q.g;
+    const int M = G.width[q.g];
+    q.total = (int64_t)N * M;
+    q.e0 = ((b - G.first_block[q.g]) * 256 + threadIdx.x) * 4;
+    if (q.e0 >= q.total) return q;
+    // (32-bit row arithmetic wherever the array allows it: a 64-bit division is a subroutine)
+    q.mask = q.total <= 0x7FFFFFFFll ? visible_quad<uint32_t>(visible, (uint32_t)q.e0, (uint32_t)q.total, M)
+                                     : visible_quad<int64_t>(visible, q.e0, q.total, M);
+    return q;
 }
 
 __device__ __forceinline__ void load_quad(const float* __restrict__ p, int64_t e0, int64_t total, float q[4]) {
@@ -161,10 +169,8 @@ __device__ __forceinline__ void load_quad(const float* __restrict__ p, int64_t e
     }
 }
 
-// Only a quad that is visible as a whole is stored with one access: the elements of invisible
-// rows are not written, not even with their own value.
-__device__ __forceinline__ void store_quad(float* __restrict__ p, int64_t e0, int m, const float q[4]) {
-    if (m == 0xF) {
+__device__ __forceinline__ void store_quad(float* __restrict__ p, int64_t e0, int64_t total, const float q[4]) {
+    if (e0 + 4 <= total) {
         quad_t v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = q[k];
@@ -172,27 +178,42 @@ __device__ __forceinline__ void store_quad(float* __restrict__ p, int64_t e0, in
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if ((m >> k) & 1) p[e0 + k] = q[k];
+            if (e0 + k < total) p[e0 + k] = q[k];
     }
 }
 
+// Four quads per lane and round: their visibility bytes, then their gradients are in flight
+// together (one at a time the two dependent loads left this at 1 TB/s).
 __global__ __launch_bounds__(256) void adam_norm_partial_kernel(AdamGroups G,
                                                                 const uint8_t* __restrict__ visible,
                                                                 int N, double* __restrict__ partial) {
     __shared__ double scratch[16];
-    double acc = 0.0;
-    for_visible_quads(G, visible, N, [&](int g, int64_t e0, int64_t total, int m) {
-        float q[4];
-        load_quad(G.grad[g], e0, total, q);
+    constexpr int U = 4;
+    double acc[U] = {0.0, 0.0, 0.0, 0.0};
+    int g = 0;
+    for (int64_t b = blockIdx.x; b < G.first_block[G.n]; b += U * (int64_t)gridDim.x) {
+        Quad q[U];
+        float d[U][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) norm_take<NORM_2>(acc, (m >> k) & 1 ? q[k] : 0.f);
-    });
-    acc = norm_join_block<NORM_2>(acc, scratch);
-    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+        for (int u = 0; u < U; ++u) q[u] = quad_of(G, visible, N, b + u * (int64_t)gridDim.x, g);
+        g = q[0].g;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (q[u].mask) load_quad(G.grad[q[u].g], q[u].e0, q[u].total, d[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) norm_take<NORM_2>(acc[u], (q[u].mask >> k) & 1 ? d[u][k] : 0.f);
+    }
+    const double v = norm_join_block<NORM_2>((acc[0] + acc[1]) + (acc[2] + acc[3]), scratch);
+    if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
+struct AdamConstants { float b1, c1, b2, c2, eps; };
+
 __global__ __launch_bounds__(256) void sparse_adam_clipped_kernel(
-    AdamGroups G, const uint8_t* __restrict__ visible, float b1, float b2, float eps, int N,
+    AdamGroups G, const uint8_t* __restrict__ visible, AdamConstants C, int N,
     const double* __restrict__ partial, int n_partial, float max_norm, float* __restrict__ norm_out,
     const uint32_t* __restrict__ guard_count, uint32_t guard_limit) {
     __shared__ double scratch[16];
@@ -201,19 +222,26 @@ __global__ __launch_bounds__(256) void sparse_adam_clipped_kernel(
     if (!(norm <= 3.402823466e+38f)) return;                    // infinite or NaN: no step
     if (guard_count && *guard_count > guard_limit) return;
     const float coef = clip_coefficient(norm, max_norm);
-    for_visible_quads(G, visible, N, [&](int g, int64_t e0, int64_t total, int m) {
+    int g = 0;
+    for (int64_t b = blockIdx.x; b < G.first_block[G.n]; b += gridDim.x) {
+        const Quad q = quad_of(G, visible, N, b, g);
+        g = q.g;
+        if (!q.mask) continue;
         float p[4], d[4], mo[4], vo[4];
-        load_quad(G.grad[g], e0, total, d);
-        load_quad(G.param[g], e0, total, p);
-        load_quad(G.m[g], e0, total, mo);
-        load_quad(G.v[g], e0, total, vo);
+        load_quad(G.grad[g], q.e0, q.total, d);
+        load_quad(G.param[g], q.e0, q.total, p);
+        load_quad(G.m[g], q.e0, q.total, mo);
+        load_quad(G.v[g], q.e0, q.total, vo);
         const float lr = G.lr[g];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) adam_update(p[k], d[k] * coef, mo[k], vo[k], lr, b1, b2, eps);
-        store_quad(G.param[g], e0, m, p);
-        store_quad(G.m[g], e0, m, mo);
-        store_quad(G.v[g], e0, m, vo);
-    });
+        for (int k = 0; k < 4; ++k) {
+            if (!((q.mask >> k) & 1)) continue;       // written back as it was
+            adam_update(p[k], d[k] * coef, mo[k], vo[k], lr, C.b1, C.c1, C.b2, C.c2, C.eps);
+        }
+        store_quad(G.param[g], q.e0, q.total, p);
+        store_quad(G.m[g], q.e0, q.total, mo);
+        store_quad(G.v[g], q.e0, q.total, vo);
+    }
 }
 
 }  // namespace vings
@@ -306,8 +334,8 @@ extern "C" size_t vings_sparse_adam_clipped_workspace_bytes(int n_groups) {
 extern "C" int vings_sparse_adam_clipped(int n_groups, float* const* params_host,
                                          const float* const* grads_host, float* const* exp_avgs_host,
                                          float* const* exp_avg_sqs_host, const int* widths_host,
-                                         const float* lrs_host, const float* b1s_host,
-                                         const float* b2s_host, const float* epss_host,
+                                         const float* lrs_host, const double* b1s_host,
+                                         const double* b2s_host, const float* epss_host,
                                          const uint8_t* visible, int N, float max_norm, float* norm,
                                          void* workspace, size_t workspace_bytes,
                                          const uint32_t* instance_count, uint32_t capacity,
@@ -368,9 +396,11 @@ extern "C" int vings_sparse_adam_clipped(int n_groups, float* const* params_host
                b2s_host[i + n] == b2s_host[i] && epss_host[i + n] == epss_host[i]) ++n;
         const int64_t blocks = table(i, n, G);
         const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(kStepBlocks, blocks));
-        sparse_adam_clipped_kernel<<<grid, 256, 0, s>>>(G, visible, b1s_host[i], b2s_host[i], epss_host[i], N,
-                                                        partial, n_partial, max_norm, i == 0 ? norm : nullptr,
-                                                        instance_count, capacity);
+        // 1 - beta is formed in 64 bits: float32(1) - float32(0.999) is 1.3e-5 off
+        const AdamConstants C{(float)b1s_host[i], (float)(1.0 - b1s_host[i]), (float)b2s_host[i],
+                              (float)(1.0 - b2s_host[i]), epss_host[i]};
+        sparse_adam_clipped_kernel<<<grid, 256, 0, s>>>(G, visible, C, N, partial, n_partial, max_norm,
+                                                        i == 0 ? norm : nullptr, instance_count, capacity);
         VINGS_LAUNCH_CHECK();
         i += n;
     }

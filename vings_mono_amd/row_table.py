@@ -63,7 +63,7 @@ def _lookup_backward(grad, ids, num_rows, scale, padding_id, out, touched, keep_
     flat = ids.contiguous()
     L, dev, et = _lib.lib(), grad.device, _lib.ELEM_TYPES[grad.dtype]
     with _lib.on_device(dev):
-        ws = torch.empty(L.vings_row_lookup_backward_workspace_bytes(n, D, et), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.vings_row_lookup_backward_workspace_bytes(n, num_rows, D, et), dtype=torch.uint8, device=dev)
         check(L.vings_row_lookup_backward(
             n, num_rows, D, src.data_ptr(), ld, et, flat.data_ptr(), flat.element_size(),
             -1 if padding_id is None else int(padding_id), scale, out.data_ptr(),

@@ -541,7 +541,8 @@ class SparseGaussianAdam(torch.optim.Adam):
         (vings_sparse_adam_clipped).  Without max_norm nothing is returned."""
         L = _lib.lib()
         _lib.require_gpu_tensor(visibility, "visibility")
-        vis = visibility.reshape(-1).to(torch.uint8).contiguous()
+        vis = visibility.reshape(-1).contiguous()
+        vis = vis.view(torch.uint8) if vis.dtype == torch.bool else vis.to(torch.uint8)
         if vis.numel() != N:
             raise _lib.VingsError("visibility must hold N entries")
         if max_norm is not None:
@@ -619,13 +620,14 @@ class SparseGaussianAdam(torch.optim.Adam):
         n = len(rows)
         if n == 0:
             return torch.zeros((), dtype=torch.float32, device=dev)
-        f = lambda k: (ctypes.c_float * n)(*[c[k] for c in consts])
+        col = lambda k, kind: (kind * n)(*[c[k] for c in consts])
         tables = [(ctypes.c_void_p * n)(*[ptr(r[k]) for r in rows]) for k in range(4)]
         with _lib.on_device(dev):
             nbytes = L.vings_sparse_adam_clipped_workspace_bytes(n)
             norm, ws = norm_and_workspace(nbytes, dev)
             check(L.vings_sparse_adam_clipped(
-                n, *tables, (ctypes.c_int * n)(*[c[0] for c in consts]), f(1), f(2), f(3), f(4),
+                n, *tables, col(0, ctypes.c_int), col(1, ctypes.c_float), col(2, ctypes.c_double),
+                col(3, ctypes.c_double), col(4, ctypes.c_float),
                 ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
                 None if guard is None else guard[0], 0 if guard is None else int(guard[1]),
                 stream_ptr(dev)), "vings_sparse_adam_clipped")

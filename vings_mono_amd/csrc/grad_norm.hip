@@ -82,7 +82,23 @@ __device__ __forceinline__ void chunk_norm(const void* in, int64_t off, int64_t 
 #pragma unroll
             for (int k = 0; k < V; ++k) norm_take<KIND>(acc[k & 3], (float)v[r][k]);
     } else {
-        for (int i = lane; i < (int)n; i += 64) norm_take<KIND>(acc[0], (float)p[i]);
+        // whole vectors, all in flight, then the up to V - 1 elements behind them
+        const int whole = (int)n / V;
+        vec v[R];
+        const int at = whole * V + lane;
+        const T rest = p[min(at, (int)n - 1)];
+        // (unguarded: a load inside a divergent branch is waited for where the branch ends)
+        if (whole > 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r] = *(const vec*)(p + min(r * 64 + lane, whole - 1) * V);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r * 64 + lane < whole) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) norm_take<KIND>(acc[k & 3], (float)v[r][k]);
+            }
+        if (at < (int)n) norm_take<KIND>(acc[0], (float)rest);
     }
 }
 
@@ -116,22 +132,34 @@ __device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t o
     O* q = (O*)out + off;
     const int lane = threadIdx.x & 63;
     const int64_t n = numel - off;
+    auto put = [&](int r, const vec& x) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            ovec o;
+#pragma unroll
+            for (int k = 0; k < OV; ++k) o[k] = (O)((float)x[s * OV + k] * coef);
+            *(ovec*)(q + (r * 64 + lane) * V + s * OV) = o;
+        }
+    };
+    vec v[R];
     if (n >= kChunk) {
-        vec v[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) v[r] = *(const vec*)(p + (r * 64 + lane) * V);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                ovec o;
-#pragma unroll
-                for (int k = 0; k < OV; ++k) o[k] = (O)((float)v[r][s * OV + k] * coef);
-                *(ovec*)(q + (r * 64 + lane) * V + s * OV) = o;
-            }
-    } else {
-        for (int i = lane; i < (int)n; i += 64) q[i] = (O)((float)p[i] * coef);
+        for (int r = 0; r < R; ++r) put(r, v[r]);
+        return;
     }
+    // whole vectors, all in flight, then the up to V - 1 elements behind them
+    const int whole = (int)n / V, at = whole * V + lane;
+    const T rest = p[min(at, (int)n - 1)];
+    if (whole > 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = *(const vec*)(p + min(r * 64 + lane, whole - 1) * V);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (r * 64 + lane < whole) put(r, v[r]);
+    if (at < (int)n) q[at] = (O)((float)rest * coef);
 }
 
 // A gradient that is already short enough stays as it is: in place, nothing is read or written.
@@ -225,10 +253,9 @@ namespace {
 
 inline int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
-// Workgroups for a launch over `chunks` chunks: two chunks per wave before a second workgroup
-// is worth its partial result, at most kMaxPartials.
+// Workgroups for a launch over `chunks` chunks: a chunk per wave, at most kMaxPartials of them.
 inline int blocks_for(int64_t chunks) {
-    return (int)std::min<int64_t>(kMaxPartials, std::max<int64_t>(1, (chunks + 7) / 8));
+    return (int)std::min<int64_t>(kMaxPartials, std::max<int64_t>(1, (chunks + 3) / 4));
 }
 
 struct ListPlan {                      // the non-empty tensors, cut into launches
@@ -400,7 +427,7 @@ extern "C" size_t vings_grad_norm_workspace_bytes(int n_tensors, const int64_t* 
         if (numels_host[i] <= 0) continue;
         const int64_t c = chunks_of(numels_host[i]);
         if (held == kClipTensors || chunks + c > 0xFFFFFFFFll) { ++launches; held = 0; chunks = 0; }
-        ++held; chunks += c; partials += c / 8 + 1;
+        ++held; chunks += c; partials += c / 4 + 1;
     }
     return sizeof(double) * (size_t)std::min<int64_t>(partials + launches, (int64_t)launches * kMaxPartials);
 }

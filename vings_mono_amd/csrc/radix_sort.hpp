@@ -51,11 +51,14 @@ static __global__ __launch_bounds__(kSortThreads) void sort_tile_hist_kernel(
     h[threadIdx.x] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * kSortTile;
+    // (unguarded loads: one inside a divergent branch is waited for where the branch ends)
+    uint32_t key[kSortItems];
 #pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        const int64_t i = base + r * kSortThreads + threadIdx.x;
-        if (i < D) atomicAdd(&h[digit_of(sort_key(keys[i], range), shift)], 1u);
-    }
+    for (int r = 0; r < kSortItems; ++r)
+        key[r] = base < D ? sort_key(keys[min(base + r * kSortThreads + threadIdx.x, D - 1)], range) : 0u;
+#pragma unroll
+    for (int r = 0; r < kSortItems; ++r)
+        if (base + r * kSortThreads + threadIdx.x < D) atomicAdd(&h[digit_of(key[r], shift)], 1u);
     __syncthreads();
     thist[(size_t)threadIdx.x * ntiles + blockIdx.x] = h[threadIdx.x];
 }
@@ -138,13 +141,20 @@ static __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
     uint32_t val[kSortItems];
     uint32_t rank[kSortItems];
     const uint64_t lt_mask = lane == 0 ? 0ull : (~0ull >> (64 - lane));
+    // (unguarded loads, see above; a speculative launch may have tiles behind the last key)
+    if ((int64_t)blockIdx.x * kSortTile < D) {
+#pragma unroll
+        for (int r = 0; r < kSortItems; ++r) {
+            const int64_t i = wbase + r * 64 + lane, at = min(i, D - 1);
+            key[r] = sort_key(keys_in[at], range);
+            if constexpr (kIds<K>) val[r] = (uint32_t)i;
+            else val[r] = vals_in[at];
+        }
+    }
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
-        const int64_t i = wbase + r * 64 + lane;
-        const bool valid = i < D;
-        key[r] = valid ? sort_key(keys_in[i], range) : ~0u;
-        if constexpr (kIds<K>) val[r] = (uint32_t)i;
-        else val[r] = valid ? vals_in[i] : 0u;
+        const bool valid = wbase + r * 64 + lane < D;
+        if (!valid) key[r] = ~0u;
         const uint32_t d = digit_of(key[r], shift);
         uint64_t peers = __ballot(valid);
 #pragma unroll

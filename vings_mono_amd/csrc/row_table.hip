@@ -41,7 +41,8 @@ namespace vings {
 constexpr int kRun = 1024;                // ids a workgroup sorts in LDS
 constexpr int kMaxRuns = 16;              // runs the merge launch takes
 constexpr int kMergeSortMax = kRun * kMaxRuns;
-constexpr int kTileIds = 1024;            // ids per workgroup of the few-rows form
+constexpr int kTileItems = 4;             // ids per lane of the few-rows form
+constexpr int kTileIds = 256 * kTileItems;
 constexpr int kFewRows = 255;             // ... one 8-bit digit, the ids without a row included
 constexpr int kFewTiles = 4096;           // ... partial rows that its join adds, at most
 constexpr int kPieceMax = 2048;           // sorted positions per workgroup of the segment kernel
@@ -84,7 +85,7 @@ __device__ __forceinline__ void store_cols(O* __restrict__ p, const float f[V]) 
     }
 }
 
-// A row per lane group of 2^LG lanes, four rows at a time; rows of up to 64 vectors.
+// A row per lane group of 2^lg lanes, four rows at a time; rows of up to 64 vectors.
 template <typename T, typename I, int V>
 __global__ __launch_bounds__(256) void row_lookup_kernel(
     int64_t N, int64_t D, const T* __restrict__ table, int64_t ld, const I* __restrict__ ids,
@@ -280,12 +281,21 @@ __global__ __launch_bounds__(kMergeThreads) void row_merge_runs_kernel(
               (int64_t)(gridDim.x - n_merge) * kMergeThreads);
         return;
     }
-    for (int i = 4 * threadIdx.x; i < n_runs * kRun; i += 4 * kMergeThreads) {
-        if (i + 4 <= N) {
-            *reinterpret_cast<uint4*>(lkey + i) = *reinterpret_cast<const uint4*>(keys + i);
-        } else {
-            for (int k = i; k < i + 4; ++k) lkey[k] = k < N ? keys[k] : ~0u;
-        }
+    // (all loads in flight together: the launch is a chain of latencies)
+    uint4 q[kMaxRuns];
+    static_assert(kRun == 4 * kMergeThreads, "a run is one round of 16-byte loads");
+#pragma unroll
+    for (int r = 0; r < kMaxRuns; ++r) {
+        // (a load that begins before N ends inside the array's 256-byte granule)
+        const int i = r * kRun + 4 * threadIdx.x;
+        q[r] = *reinterpret_cast<const uint4*>(keys + (i < N ? i : 0));
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxRuns; ++r) {
+        const int i = r * kRun + 4 * threadIdx.x;
+        const uint4 k = make_uint4(i < N ? q[r].x : ~0u, i + 1 < N ? q[r].y : ~0u, i + 2 < N ? q[r].z : ~0u,
+                                   i + 3 < N ? q[r].w : ~0u);
+        if (r < n_runs) *reinterpret_cast<uint4*>(lkey + i) = k;
     }
     __syncthreads();
     const int e = blockIdx.x * kMergeThreads + threadIdx.x;
@@ -360,44 +370,42 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const T* __restrict_
             has_head = true; head_key = cur;
 #pragma unroll
             for (int k = 0; k < V; ++k) head[k] = acc[k];
-        } else if (cur < S.rows && col_ok) {
+        } else if (col_ok) {
             write(cur, acc);
         }
     };
-    if (first < last) {
+    // ids without a row are the last ones of the order: the walk ends before them
+    int stop = last;
+    while (stop > first && skey[stop] >= S.rows) --stop;
+    if (first < stop) {
         cur = skey[first + 1];
         from_left = skey[first] == cur;
-        if (!from_left && cur < S.rows) begin(cur);
+        if (!from_left) begin(cur);
         constexpr int U = 8;
-        for (int i0 = first; i0 < last; i0 += U) {
+        for (int i0 = first; i0 < stop; i0 += U) {
+            // (lanes beyond the row's columns and positions behind the last load what is there)
             vec v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + u;
-                if (i < last && col_ok && skey[i + 1] < S.rows)
-                    v[u] = *reinterpret_cast<const vec*>(grad + (int64_t)spos[i] * S.ld + c);
-            }
+            for (int u = 0; u < U; ++u)
+                v[u] = *reinterpret_cast<const vec*>(grad + (int64_t)spos[min(i0 + u, stop - 1)] * S.ld + c);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int i = i0 + u;
-                if (i >= last) break;
-                const uint32_t k_i = skey[i + 1];
+                if (i0 + u >= stop) break;
+                const uint32_t k_i = skey[i0 + u + 1];
                 if (k_i != cur) {
                     close_run();
                     cur = k_i; from_left = false;
-                    if (cur < S.rows) begin(cur);
+                    begin(cur);
 #pragma unroll
                     for (int k = 0; k < V; ++k) acc[k] = 0.f;
                 }
-                if (col_ok && k_i < S.rows) {
-                    float f[V];
-                    unpack<T, V>(v[u], f);
+                float f[V];
+                unpack<T, V>(v[u], f);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) acc[k] += f[k];
-                }
+                for (int k = 0; k < V; ++k) acc[k] += f[k];
             }
         }
-        if (skey[last + 1] == cur) has_tail = true; else close_run();
+        if (skey[stop + 1] == cur) has_tail = true; else close_run();
     }
 
     // Open sums: inclusive scan over the groups, where a group whose positions are one single
@@ -435,11 +443,11 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const T* __restrict_
 #pragma unroll
             for (int k = 0; k < V; ++k) head[k] += sh.val[k * 256 + q];
         }
-        if (head_key < S.rows && col_ok) {
+        if (col_ok) {
             if (before_piece) write_head(head); else write(head_key, head);
         }
     }
-    if (has_tail && last == len && cur < S.rows && col_ok) write_tail(acc, open);
+    if (has_tail && last == len && col_ok) write_tail(acc, open);
 }
 
 template <typename O, int V>
@@ -505,17 +513,23 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    if (col_ok) {
-        if (g == 0) {
+    if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = S.partial[((int64_t)b * 2 + 1) * S.D + c + i];
-        }
-#pragma unroll 4
-        for (int p = 1 + g; p <= count; p += n_groups) {
-            const float* q = S.partial + ((int64_t)(b + p) * 2) * S.D + c;
+        for (int i = 0; i < V; ++i) acc[i] = S.partial[((int64_t)b * 2 + 1) * S.D + c + i];
+    }
+    constexpr int U = 4;
+    for (int p0 = 1 + g; p0 <= count; p0 += U * n_groups) {
+        float f[U][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += q[i];
+        for (int u = 0; u < U; ++u) {
+            const float* q = S.partial + ((int64_t)(b + min(p0 + u * n_groups, count)) * 2) * S.D + c;
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[u][i] = q[i];
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += p0 + u * n_groups <= count ? f[u][i] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) sval[i * 256 + threadIdx.x] = acc[i];
@@ -551,16 +565,16 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * kTileIds;
     const int len = (int)min((int64_t)kTileIds, (int64_t)S.N - first);
-    uint32_t key[4], place[4];
+    uint32_t key[kTileItems], place[kTileItems];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = (w * 4 + r) * 64 + lane;
-        key[r] = i < len ? sort_key(ids[first + i], range) : ~0u;
+    for (int r = 0; r < kTileItems; ++r) {
+        const int i = (w * kTileItems + r) * 64 + lane;
+        key[r] = sort_key(ids[first + min(i, len - 1)], range);
     }
-    block_digit_places<4, 4>(key, len, 0, bits, counts, base, wsum, place);
+    block_digit_places<4, kTileItems>(key, len, 0, bits, counts, base, wsum, place);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = (w * 4 + r) * 64 + lane;
+    for (int r = 0; r < kTileItems; ++r) {
+        const int i = (w * kTileItems + r) * 64 + lane;
         if (i < len) { skey[place[r] + 1] = key[r]; spos[place[r]] = (uint32_t)i; }
     }
     if (threadIdx.x == 0) { skey[0] = skey[len + 1] = kNoKey; base[kRadix] = (uint32_t)len; }
@@ -590,12 +604,14 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
         [](const float*) {}, [](const float*, bool) {}, [](uint32_t) {});
 }
 
-// One workgroup per row: its partial rows over the tiles, in a fixed tree.
+// One workgroup per row: its partial rows over the tiles, in a fixed tree.  The lanes of a large
+// workgroup, since the launch is two dependent loads per round whatever the rounds hold.
+constexpr int kTileJoin = 1024;
 template <typename O, int V>
-__global__ __launch_bounds__(256) void row_tile_join_kernel(Segments S, const uint8_t* __restrict__ met, int tiles,
+__global__ __launch_bounds__(kTileJoin) void row_tile_join_kernel(Segments S, const uint8_t* __restrict__ met, int tiles,
                                                             O* __restrict__ out, int keep_touched) {
-    __shared__ float sval[256 * V];
-    const int lanes = 1 << S.lg, n_groups = 256 >> S.lg;
+    __shared__ float sval[kTileJoin * V];
+    const int lanes = 1 << S.lg, n_groups = kTileJoin >> S.lg;
     const int g = threadIdx.x >> S.lg;
     const int64_t row = blockIdx.x, j = threadIdx.x & (lanes - 1);
     const bool col_ok = j * V < S.D;
@@ -613,33 +629,29 @@ __global__ __launch_bounds__(256) void row_tile_join_kernel(Segments S, const ui
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int t = t0 + u * n_groups;
-            in[u] = t < tiles && has[t];
+            in[u] = has[min(t, tiles - 1)] && t < tiles;
         }
+        // (partial rows that no tile wrote are read and not used)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[u][i] = part[(int64_t)min(t0 + u * n_groups, tiles - 1) * S.D + i];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (in[u] && col_ok) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[u][i] = part[(int64_t)(t0 + u * n_groups) * S.D + i];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (in[u] && col_ok) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] += f[u][i];
-            }
+            for (int i = 0; i < V; ++i) acc[i] += in[u] ? f[u][i] : 0.f;
             any |= in[u];
         }
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) sval[i * 256 + threadIdx.x] = acc[i];
+    for (int i = 0; i < V; ++i) sval[i * kTileJoin + threadIdx.x] = acc[i];
     any = __syncthreads_or(any);
     for (int s = n_groups >> 1; s > 0; s >>= 1) {
         if (g < s) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                acc[i] += sval[i * 256 + threadIdx.x + (s << S.lg)];
-                sval[i * 256 + threadIdx.x] = acc[i];
+                acc[i] += sval[i * kTileJoin + threadIdx.x + (s << S.lg)];
+                sval[i * kTileJoin + threadIdx.x] = acc[i];
             }
         }
         __syncthreads();
@@ -649,6 +661,9 @@ __global__ __launch_bounds__(256) void row_tile_join_kernel(Segments S, const ui
 }
 
 namespace {
+
+// clearing in a launch of its own: 64 KB per workgroup, eight workgroups per CU at most
+int clear_grid(const Fill& F) { return (int)std::min<int64_t>(2048, (F.bytes + F.n_touched + 65535) / 65536); }
 
 int ceil_log2(int64_t x) { int l = 0; while (((int64_t)1 << l) < x) ++l; return l; }
 
@@ -787,7 +802,7 @@ int few_launches(const Segments& S, const SegmentPlan& p, const GradWorkspace& w
                                                          keep_touched);
     VINGS_LAUNCH_CHECK();
     if (p.pieces > 1) {
-        row_tile_join_kernel<O, V><<<(int)S.rows, 256, 0, s>>>(S, w.met, p.pieces, (O*)out, keep_touched);
+        row_tile_join_kernel<O, V><<<(int)S.rows, kTileJoin, 0, s>>>(S, w.met, p.pieces, (O*)out, keep_touched);
         VINGS_LAUNCH_CHECK();
     }
     return VINGS_OK;
@@ -861,6 +876,7 @@ extern "C" int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, c
     if (rc != VINGS_OK) return rc;
     if (n_ids == 0) return VINGS_OK;
     VINGS_REQUIRE((table || n_rows == 0) && ids && out, "null pointer");
+
     VINGS_REQUIRE(table_stride >= n_cols || n_rows <= 1, "rows must not overlap");
     VINGS_REQUIRE((((uintptr_t)table | (uintptr_t)out) & (elem_bytes(type) - 1)) == 0 &&
                       ((uintptr_t)ids & (id_bytes - 1)) == 0, "element alignment");
@@ -896,11 +912,9 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
     VINGS_REQUIRE(((uintptr_t)rows & (elem_bytes(rows_type) - 1)) == 0, "element alignment");
     hipStream_t s = (hipStream_t)stream;
     const Fill F{rows, n_rows * n_cols * elem_bytes(rows_type), touched, touched && !keep_touched ? n_rows : 0};
-    // clearing in a launch of its own: 64 KB per workgroup, eight workgroups per CU at most
-    const int clear_blocks = (int)std::min<int64_t>(2048, (F.bytes + F.n_touched + 65535) / 65536);
     ProfScope prof(PROF_AUX, s);
     if (n_ids == 0) {
-        row_clear_kernel<<<clear_blocks, 256, 0, s>>>(F);
+        row_clear_kernel<<<clear_grid(F), 256, 0, s>>>(F);
         VINGS_LAUNCH_CHECK();
         return VINGS_OK;
     }
@@ -935,7 +949,7 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
         rs = id_bytes == 8 ? sort_runs((const int64_t*)ids, (int)n_ids, range, bits, w, F, &at, s)
                            : sort_runs((const int32_t*)ids, (int)n_ids, range, bits, w, F, &at, s);
     } else {
-        row_clear_kernel<<<clear_blocks, 256, 0, s>>>(F);
+        row_clear_kernel<<<clear_grid(F), 256, 0, s>>>(F);
         VINGS_LAUNCH_CHECK();
         rs = id_bytes == 8 ? sort_tiles((const int64_t*)ids, n_ids, range, bits, w, &at, s)
                            : sort_tiles((const int32_t*)ids, n_ids, range, bits, w, &at, s);

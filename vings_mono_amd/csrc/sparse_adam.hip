@@ -38,14 +38,13 @@ struct AdamGroups {
 };
 
 // Row of element e in an array of rows of M floats; the widths that occur are constants.
-template <typename I>
-__device__ __forceinline__ I row_of(I e, int M) {
+__device__ __forceinline__ int64_t row_of(int64_t e, int M) {
     switch (M) {
         case 1: return e;
         case 2: return e >> 1;
         case 3: return e / 3;
         case 4: return e >> 2;
-        default: return e / (I)M;
+        default: return e / M;
     }
 }
 
@@ -110,107 +109,163 @@ __global__ __launch_bounds__(256) void sparse_adam_multi_kernel(AdamGroups G,
 constexpr int kNormBlocks = 1024;      // partial results per launch
 constexpr int kStepBlocks = 2048;      // eight workgroups per CU share the reading of the partials
 constexpr int kMaxClipGroups = 64;
+constexpr int kNormQuads = 4;          // quads per lane and round of either launch: what is in
+constexpr int kStepQuads = 2;          // flight together
 
 typedef Elem<float>::vec quad_t;       // 16-byte access at any 4-byte boundary
 
-// Which of the four elements from e0 (a multiple of 4) lie in visible rows; elements at or behind
-// `total` do not.  Four elements touch four rows of one float, else two at most.
-template <typename I>
-__device__ __forceinline__ int visible_quad(const uint8_t* __restrict__ visible, I e0, I total, int M) {
-    const int n = total - e0 >= 4 ? 4 : (int)(total - e0);
-    if (M == 1) {
-        int m = 0;
-        if (n == 4) {
-            typedef uint8_t u8x4 __attribute__((ext_vector_type(4), aligned(1)));
-            const u8x4 v = *reinterpret_cast<const u8x4*>(visible + e0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m |= v[k] ? 1 << k : 0;
-        } else {
-            for (int k = 0; k < n; ++k) m |= visible[e0 + k] ? 1 << k : 0;
-        }
-        return m;
+// Which of the four elements from e0 (a multiple of 4, e0 + 4 <= N * width) lie in visible rows of
+// W floats (W = 0: of `width` floats).  Four elements touch four rows of one float, else two at
+// most; the loads are not guarded (see below), the second row is clamped instead.
+template <int W, typename I>
+__device__ __forceinline__ int visible_quad(const uint8_t* __restrict__ visible, I e0, int N, int width) {
+    if (W == 1) {
+        typedef uint32_t u32u __attribute__((aligned(1)));
+        const uint32_t v = *reinterpret_cast<const u32u*>(visible + e0);
+        return (v & 0xFFu ? 1 : 0) | (v & 0xFF00u ? 2 : 0) | (v & 0xFF0000u ? 4 : 0) | (v >> 24 ? 8 : 0);
     }
-    const I r = row_of<I>(e0, M);
-    const I left = (r + 1) * (I)M - e0;               // elements of row r from e0 on
+    const I M = W ? (I)W : (I)width;
+    const I r = e0 / M;
+    if (W == 4) return visible[r] ? 0xF : 0;
+    const I left = (r + 1) * M - e0;                  // elements of row r from e0 on
     const int low = left >= 4 ? 0xF : (1 << (int)left) - 1;
-    int m = visible[r] ? low : 0;
-    if (left < (I)n && visible[r + 1]) m |= 0xF & ~low;
-    return m & ((1 << n) - 1);
+    const uint8_t a = visible[r], b = visible[r + 1 < (I)N ? r + 1 : r];
+    return (a ? low : 0) | (b ? 0xF & ~low : 0);
 }
 
-// A quad of one group's arrays: where it starts, and which of its elements are stepped.
-struct Quad { int g, mask; int64_t e0, total; };
-
-// The quad of this lane in block b of the launch's quads (256 consecutive ones of one group);
-// mask 0 behind the end.  `g` is a hint: a group that does not lie behind b's.
-__device__ __forceinline__ Quad quad_of(const AdamGroups& G, const uint8_t* __restrict__ visible, int N,
-                                        int64_t b, int g) {
-    Quad q{g, 0, 0, 0};
-    if (b >= G.first_block[G.n]) return q;
-    while (b >= G.first_block[q.g + 1]) ++q.g;
-    const int M = G.width[q.g];
-    q.total = (int64_t)N * M;
-    q.e0 = ((b - G.first_block[q.g]) * 256 + threadIdx.x) * 4;
-    if (q.e0 >= q.total) return q;
-    // (32-bit row arithmetic wherever the array allows it: a 64-bit division is a subroutine)
-    q.mask = q.total <= 0x7FFFFFFFll ? visible_quad<uint32_t>(visible, (uint32_t)q.e0, (uint32_t)q.total, M)
-                                     : visible_quad<int64_t>(visible, q.e0, q.total, M);
-    return q;
-}
-
-__device__ __forceinline__ void load_quad(const float* __restrict__ p, int64_t e0, int64_t total, float q[4]) {
-    if (e0 + 4 <= total) {
-        const quad_t v = *reinterpret_cast<const quad_t*>(p + e0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = v[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = e0 + k < total ? p[e0 + k] : 0.f;
+// What a launch does with the arrays of one group: block<W, I>(group, first quad, quads) serves
+// 256 * quads-per-lane quads of four elements, tail(group, e0, n) the up to three elements behind
+// the last whole quad, one lane each.
+//
+// All loads of a block are issued for every lane, lanes behind the end taking the last quad again:
+// a load inside a divergent branch is waited for where the branch ends, and a lane's loads then
+// follow one another instead of being in flight together (norm of 1 M splats 26 -> NORM_US us).
+// The row widths of a splat map are constants, and indexes have 32 bits wherever the arrays
+// allow it (a 64-bit division is a subroutine).
+template <typename F>
+__device__ __forceinline__ void for_blocks(const AdamGroups& G, int N, int per_lane, F f) {
+    int g = 0;
+    for (int64_t b = blockIdx.x; b < G.first_block[G.n]; b += gridDim.x) {
+        while (b >= G.first_block[g + 1]) ++g;
+        const int64_t total = (int64_t)N * G.width[g], quads = total >> 2;
+        const int64_t first = (b - G.first_block[g]) * 256 * per_lane;
+        if (first < quads) {
+            if (total > 0x7FFFFFFFll - 8192) {
+                f.template block<0, int64_t>(g, first, quads);
+            } else {
+                const uint32_t f32 = (uint32_t)first, q32 = (uint32_t)quads;
+                switch (G.width[g]) {
+                    case 1: f.template block<1, uint32_t>(g, f32, q32); break;
+                    case 2: f.template block<2, uint32_t>(g, f32, q32); break;
+                    case 3: f.template block<3, uint32_t>(g, f32, q32); break;
+                    case 4: f.template block<4, uint32_t>(g, f32, q32); break;
+                    default: f.template block<0, uint32_t>(g, f32, q32); break;
+                }
+            }
+        }
+        // (the last block of a group; it exists for the tail alone where total < 4)
+        if ((total & 3) && first + 256 * per_lane > quads && (int)threadIdx.x < (int)(total & 3))
+            f.tail(g, quads * 4 + threadIdx.x);
     }
 }
 
-__device__ __forceinline__ void store_quad(float* __restrict__ p, int64_t e0, int64_t total, const float q[4]) {
-    if (e0 + 4 <= total) {
-        quad_t v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = q[k];
-        *reinterpret_cast<quad_t*>(p + e0) = v;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (e0 + k < total) p[e0 + k] = q[k];
-    }
-}
+struct SquareSum {
+    const AdamGroups& G;
+    const uint8_t* __restrict__ visible;
+    int N;
+    double (&acc)[kNormQuads];
 
-// Four quads per lane and round: their visibility bytes, then their gradients are in flight
-// together (one at a time the two dependent loads left this at 1 TB/s).
+    template <int W, typename I>
+    __device__ __forceinline__ void block(int g, I first, I quads) {
+        int mask[kNormQuads];
+        quad_t d[kNormQuads];
+        const float* __restrict__ grad = G.grad[g];
+#pragma unroll
+        for (int u = 0; u < kNormQuads; ++u) {
+            const I q = first + u * 256 + threadIdx.x, e0 = (q < quads ? q : quads - 1) * 4;
+            d[u] = *reinterpret_cast<const quad_t*>(grad + e0);
+            mask[u] = visible_quad<W, I>(visible, e0, N, G.width[g]);
+        }
+#pragma unroll
+        for (int u = 0; u < kNormQuads; ++u) {
+            const int m = first + u * 256 + threadIdx.x < quads ? mask[u] : 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) norm_take<NORM_2>(acc[u], (m >> k) & 1 ? d[u][k] : 0.f);
+        }
+    }
+    __device__ __forceinline__ void tail(int g, int64_t e) {
+        if (visible[e / G.width[g]]) norm_take<NORM_2>(acc[0], G.grad[g][e]);
+    }
+};
+
 __global__ __launch_bounds__(256) void adam_norm_partial_kernel(AdamGroups G,
                                                                 const uint8_t* __restrict__ visible,
                                                                 int N, double* __restrict__ partial) {
     __shared__ double scratch[16];
-    constexpr int U = 4;
-    double acc[U] = {0.0, 0.0, 0.0, 0.0};
-    int g = 0;
-    for (int64_t b = blockIdx.x; b < G.first_block[G.n]; b += U * (int64_t)gridDim.x) {
-        Quad q[U];
-        float d[U][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = quad_of(G, visible, N, b + u * (int64_t)gridDim.x, g);
-        g = q[0].g;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (q[u].mask) load_quad(G.grad[q[u].g], q[u].e0, q[u].total, d[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) norm_take<NORM_2>(acc[u], (q[u].mask >> k) & 1 ? d[u][k] : 0.f);
-    }
+    double acc[kNormQuads] = {};
+    for_blocks(G, N, kNormQuads, SquareSum{G, visible, N, acc});
     const double v = norm_join_block<NORM_2>((acc[0] + acc[1]) + (acc[2] + acc[3]), scratch);
     if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
 struct AdamConstants { float b1, c1, b2, c2, eps; };
+
+struct ClippedUpdate {
+    const AdamGroups& G;
+    const uint8_t* __restrict__ visible;
+    int N;
+    AdamConstants C;
+    float coef;
+
+    template <int W, typename I>
+    __device__ __forceinline__ void block(int g, I first, I quads) {
+        int mask[kStepQuads], any = 0;
+        quad_t p[kStepQuads], d[kStepQuads], m[kStepQuads], v[kStepQuads];
+        I e0[kStepQuads];
+#pragma unroll
+        for (int u = 0; u < kStepQuads; ++u) {
+            const I q = first + u * 256 + threadIdx.x;
+            e0[u] = (q < quads ? q : quads - 1) * 4;
+            mask[u] = visible_quad<W, I>(visible, e0[u], N, G.width[g]);
+        }
+#pragma unroll
+        for (int u = 0; u < kStepQuads; ++u) {
+            if (first + u * 256 + threadIdx.x >= quads) mask[u] = 0;
+            any |= mask[u];
+        }
+        if (__ballot(any) == 0) return;               // nothing of this wave's quads is stepped
+#pragma unroll
+        for (int u = 0; u < kStepQuads; ++u) {
+            d[u] = *reinterpret_cast<const quad_t*>(G.grad[g] + e0[u]);
+            p[u] = *reinterpret_cast<const quad_t*>(G.param[g] + e0[u]);
+            m[u] = *reinterpret_cast<const quad_t*>(G.m[g] + e0[u]);
+            v[u] = *reinterpret_cast<const quad_t*>(G.v[g] + e0[u]);
+        }
+        const float lr = G.lr[g];
+#pragma unroll
+        for (int u = 0; u < kStepQuads; ++u) {
+            if (!mask[u]) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float pk = p[u][k], mk = m[u][k], vk = v[u][k];
+                adam_update(pk, d[u][k] * coef, mk, vk, lr, C.b1, C.c1, C.b2, C.c2, C.eps);
+                const bool step = (mask[u] >> k) & 1;  // else written back as it was
+                p[u][k] = step ? pk : p[u][k];
+                m[u][k] = step ? mk : m[u][k];
+                v[u][k] = step ? vk : v[u][k];
+            }
+            *reinterpret_cast<quad_t*>(G.param[g] + e0[u]) = p[u];
+            *reinterpret_cast<quad_t*>(G.m[g] + e0[u]) = m[u];
+            *reinterpret_cast<quad_t*>(G.v[g] + e0[u]) = v[u];
+        }
+    }
+    __device__ __forceinline__ void tail(int g, int64_t e) {
+        if (!visible[e / G.width[g]]) return;
+        float p = G.param[g][e], m = G.m[g][e], v = G.v[g][e];
+        adam_update(p, G.grad[g][e] * coef, m, v, G.lr[g], C.b1, C.c1, C.b2, C.c2, C.eps);
+        G.param[g][e] = p; G.m[g][e] = m; G.v[g][e] = v;
+    }
+};
 
 __global__ __launch_bounds__(256) void sparse_adam_clipped_kernel(
     AdamGroups G, const uint8_t* __restrict__ visible, AdamConstants C, int N,
@@ -221,27 +276,7 @@ __global__ __launch_bounds__(256) void sparse_adam_clipped_kernel(
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     if (!(norm <= 3.402823466e+38f)) return;                    // infinite or NaN: no step
     if (guard_count && *guard_count > guard_limit) return;
-    const float coef = clip_coefficient(norm, max_norm);
-    int g = 0;
-    for (int64_t b = blockIdx.x; b < G.first_block[G.n]; b += gridDim.x) {
-        const Quad q = quad_of(G, visible, N, b, g);
-        g = q.g;
-        if (!q.mask) continue;
-        float p[4], d[4], mo[4], vo[4];
-        load_quad(G.grad[g], q.e0, q.total, d);
-        load_quad(G.param[g], q.e0, q.total, p);
-        load_quad(G.m[g], q.e0, q.total, mo);
-        load_quad(G.v[g], q.e0, q.total, vo);
-        const float lr = G.lr[g];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (!((q.mask >> k) & 1)) continue;       // written back as it was
-            adam_update(p[k], d[k] * coef, mo[k], vo[k], lr, C.b1, C.c1, C.b2, C.c2, C.eps);
-        }
-        store_quad(G.param[g], q.e0, q.total, p);
-        store_quad(G.m[g], q.e0, q.total, mo);
-        store_quad(G.v[g], q.e0, q.total, vo);
-    }
+    for_blocks(G, N, kStepQuads, ClippedUpdate{G, visible, N, C, clip_coefficient(norm, max_norm)});
 }
 
 }  // namespace vings
@@ -364,7 +399,7 @@ extern "C" int vings_sparse_adam_clipped(int n_groups, float* const* params_host
     double* partial = (double*)workspace;
     // one run of up to 8 consecutive groups per launch; an update launch also ends where the
     // next group has other constants
-    auto table = [&](int first, int n, AdamGroups& G) {
+    auto table = [&](int first, int n, int quads, AdamGroups& G) {
         int64_t blocks = 0;
         G.n = n;
         for (int k = 0; k < n; ++k) {
@@ -373,18 +408,18 @@ extern "C" int vings_sparse_adam_clipped(int n_groups, float* const* params_host
             G.m[k] = exp_avgs_host[i]; G.v[k] = exp_avg_sqs_host[i];
             G.width[k] = widths_host[i]; G.lr[k] = lrs_host[i];
             G.first_block[k] = (int)blocks;
-            blocks += ((int64_t)N * widths_host[i] + 1023) / 1024;
-            if (blocks > 0x7FFFFFFF - kStepBlocks) return (int64_t)-1;
+            blocks += ((int64_t)N * widths_host[i] + 1024 * quads - 1) / (1024 * quads);
+            if (blocks > 0x7FFFFFFF) return (int64_t)-1;
         }
         G.first_block[n] = (int)blocks;
         return blocks;
     };
     AdamGroups G;
     for (int i = 0; i < n_groups; i += kMaxGroups)
-        VINGS_REQUIRE(table(i, std::min(kMaxGroups, n_groups - i), G) >= 0, "groups too large");
+        VINGS_REQUIRE(table(i, std::min(kMaxGroups, n_groups - i), kStepQuads, G) >= 0, "groups too large");
     int n_partial = 0;
     for (int i = 0; i < n_groups; i += kMaxGroups) {
-        const int64_t blocks = table(i, std::min(kMaxGroups, n_groups - i), G);
+        const int64_t blocks = table(i, std::min(kMaxGroups, n_groups - i), kNormQuads, G);
         const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(kNormBlocks, blocks));
         adam_norm_partial_kernel<<<grid, 256, 0, s>>>(G, visible, N, partial + n_partial);
         VINGS_LAUNCH_CHECK();
@@ -394,7 +429,7 @@ extern "C" int vings_sparse_adam_clipped(int n_groups, float* const* params_host
         int n = 1;
         while (n < kMaxGroups && i + n < n_groups && b1s_host[i + n] == b1s_host[i] &&
                b2s_host[i + n] == b2s_host[i] && epss_host[i + n] == epss_host[i]) ++n;
-        const int64_t blocks = table(i, n, G);
+        const int64_t blocks = table(i, n, kStepQuads, G);
         const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(kStepBlocks, blocks));
         // 1 - beta is formed in 64 bits: float32(1) - float32(0.999) is 1.3e-5 off
         const AdamConstants C{(float)b1s_host[i], (float)(1.0 - b1s_host[i]), (float)b2s_host[i],

@@ -595,33 +595,38 @@ class SparseGaussianAdam(torch.optim.Adam):
         if not max_norm >= 0.0:
             raise _lib.VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
         dev = vis.device
-        rows, consts = [], []
+        arrays, keep, consts = [], [], []
         for group in self.param_groups:
             if len(group["params"]) != 1:
                 raise _lib.VingsError("more than one tensor in group")
             p = group["params"][0]
-            if p.grad is None:
+            g = p.grad
+            if g is None:
                 continue
             _lib.require_gpu_tensor(p, "param", torch.float32)
-            if p.device != dev:
-                raise _lib.VingsError("parameters and visibility must live on one device")
-            if p.grad.dtype != torch.float32:
-                raise _lib.VingsError(f"gradients must be float32 (got {p.grad.dtype})")
-            if N == 0:
+            if p.device != dev or g.device != dev:
+                raise _lib.VingsError("parameters, gradients and visibility must live on one device")
+            if g.dtype != torch.float32:
+                raise _lib.VingsError(f"gradients must be float32 (got {g.dtype})")
+            size = p.numel()
+            if N == 0 or size == 0:
                 continue
-            if p.numel() % N != 0:
+            if size % N != 0:
                 raise _lib.VingsError("parameter size is not a multiple of N")
-            if p.numel() == 0:
-                continue
             state = self._moments(p)
+            g = g.contiguous()
+            keep.append(g)
+            for t in (p, g, state["exp_avg"], state["exp_avg_sq"]):
+                if not t.is_contiguous() or t.numel() != size:
+                    raise _lib.VingsError("parameters and moments must be dense and of one size")
+                arrays.append(t.data_ptr())
             b1, b2 = group.get("betas", (0.9, 0.999))
-            rows.append((p, p.grad.contiguous(), state["exp_avg"], state["exp_avg_sq"]))
-            consts.append((p.numel() // N, float(group["lr"]), float(b1), float(b2), float(group["eps"])))
-        n = len(rows)
+            consts.append((size // N, group["lr"], b1, b2, group["eps"]))
+        n = len(consts)
         if n == 0:
             return torch.zeros((), dtype=torch.float32, device=dev)
         col = lambda k, kind: (kind * n)(*[c[k] for c in consts])
-        tables = [(ctypes.c_void_p * n)(*[ptr(r[k]) for r in rows]) for k in range(4)]
+        tables = [(ctypes.c_void_p * n)(*arrays[k::4]) for k in range(4)]
         with _lib.on_device(dev):
             nbytes = L.vings_sparse_adam_clipped_workspace_bytes(n)
             norm, ws = norm_and_workspace(nbytes, dev)

@@ -121,25 +121,23 @@ __device__ __forceinline__ double range_norm(const TensorTable<CAP, OUT>& T, uin
     return norm_join<KIND>(norm_join<KIND>(acc[0], acc[1]), norm_join<KIND>(acc[2], acc[3]));
 }
 
+// The wider side sets the vector: 16 bytes of it per lane, so that its accesses are contiguous
+// over the lanes (16-bit gradients into float32: loads of 8 bytes).
 template <typename T, typename O>
 __device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t off, int64_t numel,
                                             float coef) {
-    constexpr int V = Elem<T>::kVec, R = kChunk / (64 * V);
-    typedef typename Elem<T>::vec vec;
+    constexpr int V = Elem<O>::kVec, R = kChunk / (64 * V);
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     typedef typename Elem<O>::vec ovec;
-    constexpr int OV = Elem<O>::kVec, S = V / OV;      // S output vectors per input vector
     const T* p = (const T*)in + off;
     O* q = (O*)out + off;
     const int lane = threadIdx.x & 63;
     const int64_t n = numel - off;
     auto put = [&](int r, const vec& x) {
+        ovec o;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            ovec o;
-#pragma unroll
-            for (int k = 0; k < OV; ++k) o[k] = (O)((float)x[s * OV + k] * coef);
-            *(ovec*)(q + (r * 64 + lane) * V + s * OV) = o;
-        }
+        for (int k = 0; k < V; ++k) o[k] = (O)((float)x[k] * coef);
+        *(ovec*)(q + (r * 64 + lane) * V) = o;
     };
     vec v[R];
     if (n >= kChunk) {

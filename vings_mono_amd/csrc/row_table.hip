@@ -342,19 +342,21 @@ struct Segments {
 
 // Sums of the runs of equal keys among a workgroup's `len` sorted positions.  skey[1 .. len]: the
 // keys, skey[0] and skey[len + 1] those before and behind them (kNoKey where there are none);
-// spos: the gradient rows.  Calls write(row, sum) for runs that lie inside, head(sum) for the one
-// that began before, tail(sum, all) for the one that goes on behind (all: and began before), and
-// begin(row) where a run begins; every call comes from the lanes that hold the sum's columns.
+// load(i): this lane's columns of the gradient row at position i.  Calls write(row, sum) for runs
+// that lie inside, write_head(sum) for the one that began before, write_tail(sum, all) for the one
+// that goes on behind (all: and began before), from the lanes that hold the sum's columns.
+// A wave walks several groups at once and one of them closes a run at nearly every step, so a
+// step has little to do beside its addition: the loads need no guard and the address of a row is
+// one multiply-add.
 constexpr uint32_t kNoKey = ~0u;                     // rows < 2^31
 template <int V> struct RunShared {
     float val[256 * V];                              // open sums, lane-contiguous per component
     uint8_t open[256];                               // a group's open sum reaches the left edge
 };
 
-template <typename T, int V, typename W, typename H, typename L, typename B>
-__device__ __forceinline__ void sum_runs(const Segments& S, const T* __restrict__ grad, const uint32_t* skey,
-                                         const uint32_t* spos, int len, bool col_ok, int64_t c,
-                                         RunShared<V>& sh, W write, H write_head, L write_tail, B begin) {
+template <typename T, int V, typename F, typename W, typename H, typename L>
+__device__ __forceinline__ void sum_runs(const Segments& S, const uint32_t* skey, int len, bool col_ok,
+                                         RunShared<V>& sh, F load, W write, H write_head, L write_tail) {
     typedef typename VecOf<T, V>::type vec;
     const int lanes = 1 << S.lg, n_groups = 256 >> S.lg;
     const int g = threadIdx.x >> S.lg;
@@ -377,34 +379,37 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const T* __restrict_
     // ids without a row are the last ones of the order: the walk ends before them
     int stop = last;
     while (stop > first && skey[stop] >= S.rows) --stop;
+    constexpr int U = 4;
+    auto batch = [&](int i0, int n) {              // n <= U positions from i0
+        vec v[U];
+        uint32_t key[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + min(u, n - 1);      // (a short batch loads its last row again)
+            v[u] = load(i);
+            key[u] = skey[i + 1];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= n) break;
+            if (key[u] != cur) {
+                close_run();
+                cur = key[u]; from_left = false;
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] = 0.f;
+            }
+            float f[V];
+            unpack<T, V>(v[u], f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += f[k];
+        }
+    };
     if (first < stop) {
         cur = skey[first + 1];
         from_left = skey[first] == cur;
-        if (!from_left) begin(cur);
-        constexpr int U = 8;
-        for (int i0 = first; i0 < stop; i0 += U) {
-            // (lanes beyond the row's columns and positions behind the last load what is there)
-            vec v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                v[u] = *reinterpret_cast<const vec*>(grad + (int64_t)spos[min(i0 + u, stop - 1)] * S.ld + c);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i0 + u >= stop) break;
-                const uint32_t k_i = skey[i0 + u + 1];
-                if (k_i != cur) {
-                    close_run();
-                    cur = k_i; from_left = false;
-                    begin(cur);
-#pragma unroll
-                    for (int k = 0; k < V; ++k) acc[k] = 0.f;
-                }
-                float f[V];
-                unpack<T, V>(v[u], f);
-#pragma unroll
-                for (int k = 0; k < V; ++k) acc[k] += f[k];
-            }
-        }
+        int i0 = first;
+        for (; i0 + U <= stop; i0 += U) batch(i0, U);
+        if (i0 < stop) batch(i0, stop - i0);
         if (skey[stop + 1] == cur) has_tail = true; else close_run();
     }
 
@@ -450,6 +455,9 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const T* __restrict_
     if (has_tail && last == len && col_ok) write_tail(acc, open);
 }
 
+// Byte offset of row `row` of rows that lie `pitch` bytes apart.
+__device__ __forceinline__ int64_t row_offset(uint32_t row, uint32_t pitch) { return (int64_t)((uint64_t)row * pitch); }
+
 template <typename O, int V>
 __device__ __forceinline__ void write_scaled(O* __restrict__ p, const float f[V], float scale) {
     float o[V];
@@ -461,6 +469,7 @@ __device__ __forceinline__ void write_scaled(O* __restrict__ p, const float f[V]
 template <typename T, typename O, int V>
 __global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* __restrict__ grad,
                                                           O* __restrict__ out) {
+    typedef typename VecOf<T, V>::type vec;
     extern __shared__ uint32_t smem[];                // (the usual piece takes a few hundred bytes)
     __shared__ RunShared<V> sh;
     const int lanes = 1 << S.lg;
@@ -479,12 +488,19 @@ __global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* _
     for (int i = threadIdx.x; i < len; i += 256) spos[i] = S.pos[base + i];
     __syncthreads();
     float* partial = S.partial + (int64_t)blockIdx.x * 2 * S.D + c;
+    const char* from = reinterpret_cast<const char*>(grad + c);
+    char* to = reinterpret_cast<char*>(out + c);
+    const uint32_t pitch = (uint32_t)S.ld * sizeof(T), out_pitch = (uint32_t)S.D * sizeof(O);
+    uint8_t* touched = j == 0 ? S.touched : nullptr;
     sum_runs<T, V>(
-        S, grad, skey, spos, len, col_ok, c, sh,
-        [&](uint32_t row, const float* f) { write_scaled<O, V>(out + (int64_t)row * S.D + c, f, S.scale); },
+        S, skey, len, col_ok, sh,
+        [&](int i) { return *reinterpret_cast<const vec*>(from + row_offset(spos[i], pitch)); },
+        [&](uint32_t row, const float* f) {
+            write_scaled<O, V>(reinterpret_cast<O*>(to + row_offset(row, out_pitch)), f, S.scale);
+            if (touched) touched[row] = 1;
+        },
         [&](const float* f) { store_cols<float, V>(partial, f); },
-        [&](const float* f, bool all) { store_cols<float, V>(partial + (all ? 0 : S.D), f); },
-        [&](uint32_t row) { if (S.touched && j == 0) S.touched[row] = 1; });
+        [&](const float* f, bool all) { store_cols<float, V>(partial + (all ? 0 : S.D), f); });
 }
 
 // One workgroup per piece and column segment; those in whose piece no run begins that goes on
@@ -543,7 +559,10 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
             }
         }
     }
-    if (g == 0 && col_ok) write_scaled<O, V>(out + (int64_t)k * S.D + c, acc, S.scale);
+    if (g == 0 && col_ok) {
+        write_scaled<O, V>(out + (int64_t)k * S.D + c, acc, S.scale);
+        if (S.touched && j == 0) S.touched[k] = 1;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -552,7 +571,7 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
 // The workgroup's own stable order of its 1024 ids, then their runs.  With one workgroup the sums
 // are the rows themselves; otherwise row r of tile t goes to partial[r][t], met[r][t] says
 // whether the tile has it.
-template <typename T, typename O, typename I, int V>
+template <typename T, typename O, typename I, int V, bool ALONE>
 __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __restrict__ grad,
                                                        const I* __restrict__ ids, IdRange range, int bits,
                                                        O* __restrict__ out, uint8_t* __restrict__ met,
@@ -560,8 +579,10 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
     __shared__ uint16_t counts[4][kRadix];
     __shared__ uint32_t base[kRadix + 1], wsum[4];
     __shared__ uint32_t skey[kTileIds + 2];
-    __shared__ uint32_t spos[kTileIds];
+    __shared__ uint32_t spos[kTileIds];               // byte offsets of the rows inside the tile
     __shared__ RunShared<V> sh;
+    typedef typename VecOf<T, V>::type vec;
+    const uint32_t pitch = (uint32_t)S.ld * sizeof(T);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * kTileIds;
     const int len = (int)min((int64_t)kTileIds, (int64_t)S.N - first);
@@ -575,33 +596,38 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
 #pragma unroll
     for (int r = 0; r < kTileItems; ++r) {
         const int i = (w * kTileItems + r) * 64 + lane;
-        if (i < len) { skey[place[r] + 1] = key[r]; spos[place[r]] = (uint32_t)i; }
+        if (i < len) { skey[place[r] + 1] = key[r]; spos[place[r]] = (uint32_t)i * pitch; }
     }
     if (threadIdx.x == 0) { skey[0] = skey[len + 1] = kNoKey; base[kRadix] = (uint32_t)len; }
     __syncthreads();
-    const bool alone = gridDim.x == 1;
     const int64_t tiles = gridDim.x;
     for (uint32_t r = threadIdx.x; r < S.rows; r += 256) {
         const uint8_t any = base[r + 1] > base[r];
-        if (!alone) met[r * tiles + blockIdx.x] = any;
+        if (!ALONE) met[r * tiles + blockIdx.x] = any;
         else if (S.touched && (any || !keep_touched)) S.touched[r] = any;
     }
     const int lanes = 1 << S.lg;
     const int64_t j = threadIdx.x & (lanes - 1);
     const bool col_ok = j * V < S.D;
     const int64_t c = col_ok ? vec_col<V>(j, S.D) : 0;
-    if (alone && col_ok) {
+    if (ALONE && col_ok) {
         const float zero[V] = {};
         for (uint32_t r = threadIdx.x >> S.lg; r < S.rows; r += 256 >> S.lg)
             if (base[r + 1] == base[r]) store_cols<O, V>(out + (int64_t)r * S.D + c, zero);
     }
+    const char* from = reinterpret_cast<const char*>(grad + first * S.ld + c);
+    // rows of the result, or this tile's places among the partial rows
+    char* to = ALONE ? reinterpret_cast<char*>(out + c)
+                     : reinterpret_cast<char*>(S.partial + blockIdx.x * S.D + c);
+    const uint32_t out_pitch = ALONE ? (uint32_t)S.D * sizeof(O) : (uint32_t)(tiles * S.D) * 4u;
     sum_runs<T, V>(
-        S, grad + first * S.ld, skey, spos, len, col_ok, c, sh,
+        S, skey, len, col_ok, sh, [&](int i) { return *reinterpret_cast<const vec*>(from + spos[i]); },
         [&](uint32_t row, const float* f) {
-            if (alone) write_scaled<O, V>(out + (int64_t)row * S.D + c, f, S.scale);
-            else store_cols<float, V>(S.partial + (row * tiles + blockIdx.x) * S.D + c, f);
+            char* q = to + row_offset(row, out_pitch);
+            if constexpr (ALONE) write_scaled<O, V>(reinterpret_cast<O*>(q), f, S.scale);
+            else store_cols<float, V>(reinterpret_cast<float*>(q), f);
         },
-        [](const float*) {}, [](const float*, bool) {}, [](uint32_t) {});
+        [](const float*) {}, [](const float*, bool) {});
 }
 
 // One workgroup per row: its partial rows over the tiles, in a fixed tree.  The lanes of a large
@@ -677,8 +703,7 @@ SegmentPlan plan_segments(int64_t N, int64_t rows, int64_t D, int type) {
     p.lg = vectors >= 64 ? 6 : ceil_log2(vectors);
     p.segments = (int)((vectors + (1 << p.lg) - 1) >> p.lg);
     const int groups = 256 >> p.lg;
-    // few rows: one digit, a lane group of the tile sums at most 64 positions, the partial rows
-    // stay below a quarter of the gradient
+    // few rows: one digit, a lane group of the tile sums at most 64 positions
     p.few = rows <= kFewRows && vectors <= 16 && N <= (int64_t)kFewTiles * kTileIds;
     if (p.few) {
         p.per_group = (int)((std::min<int64_t>(N, kTileIds) + groups - 1) / groups);
@@ -798,8 +823,12 @@ int segment_launches(const Segments& S, const SegmentPlan& p, const void* grad, 
 template <typename T, typename O, typename I, int V>
 int few_launches(const Segments& S, const SegmentPlan& p, const GradWorkspace& w, const void* grad, const void* ids,
                  IdRange range, int bits, void* out, int keep_touched, hipStream_t s) {
-    row_tile_kernel<T, O, I, V><<<p.pieces, 256, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out, w.met,
-                                                         keep_touched);
+    if (p.pieces == 1)
+        row_tile_kernel<T, O, I, V, true><<<1, 256, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out, w.met,
+                                                            keep_touched);
+    else
+        row_tile_kernel<T, O, I, V, false><<<p.pieces, 256, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out,
+                                                                    w.met, keep_touched);
     VINGS_LAUNCH_CHECK();
     if (p.pieces > 1) {
         row_tile_join_kernel<O, V><<<(int)S.rows, kTileJoin, 0, s>>>(S, w.met, p.pieces, (O*)out, keep_touched);
@@ -919,7 +948,7 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
         return VINGS_OK;
     }
     VINGS_REQUIRE(grad && ids, "null pointer");
-    VINGS_REQUIRE(grad_stride >= 0, "sizes");
+    VINGS_REQUIRE(grad_stride >= 0 && grad_stride < (1 << 22), "gradient rows lie less than 2^22 elements apart");
     VINGS_REQUIRE(((uintptr_t)grad & (elem_bytes(type) - 1)) == 0 && ((uintptr_t)ids & (id_bytes - 1)) == 0,
                   "element alignment");
     VINGS_REQUIRE(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");

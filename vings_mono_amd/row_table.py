@@ -16,7 +16,7 @@ def _rows_2d(t, name):
     """t [..., D] as rows with unit column stride: (tensor, number of rows, row stride)."""
     D = t.shape[-1]
     n = t.numel() // D if D else 0
-    if t.dim() == 2 and (t.stride(1) == 1 or D == 1) and (n <= 1 or t.stride(0) >= D or t.stride(0) == 0):
+    if t.dim() == 2 and (t.stride(1) == 1 or D == 1) and (n <= 1 or D <= t.stride(0) < 1 << 22 or t.stride(0) == 0):
         return t, n, t.stride(0) if n > 1 else D
     t = t.contiguous()
     return t, n, D

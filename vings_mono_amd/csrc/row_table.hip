@@ -41,8 +41,9 @@ namespace vings {
 constexpr int kRun = 1024;                // ids a workgroup sorts in LDS
 constexpr int kMaxRuns = 16;              // runs the merge launch takes
 constexpr int kMergeSortMax = kRun * kMaxRuns;
-constexpr int kTileItems = 4;             // ids per lane of the few-rows form
-constexpr int kTileIds = 256 * kTileItems;
+constexpr int kTileThreads = 512;         // few-rows form: lanes and
+constexpr int kTileIds = 1024;            // ids per workgroup
+constexpr int kTileItems = kTileIds / kTileThreads;
 constexpr int kFewRows = 255;             // ... one 8-bit digit, the ids without a row included
 constexpr int kFewTiles = 4096;           // ... partial rows that its join adds, at most
 constexpr int kPieceMax = 2048;           // sorted positions per workgroup of the segment kernel
@@ -349,16 +350,16 @@ struct Segments {
 // step has little to do beside its addition: the loads need no guard and the address of a row is
 // one multiply-add.
 constexpr uint32_t kNoKey = ~0u;                     // rows < 2^31
-template <int V> struct RunShared {
-    float val[256 * V];                              // open sums, lane-contiguous per component
-    uint8_t open[256];                               // a group's open sum reaches the left edge
+template <int V, int THREADS> struct RunShared {
+    float val[THREADS * V];                          // open sums, lane-contiguous per component
+    uint8_t open[THREADS];                           // a group's open sum reaches the left edge
 };
 
-template <typename T, int V, typename F, typename W, typename H, typename L>
+template <typename T, int V, int THREADS, typename F, typename W, typename H, typename L>
 __device__ __forceinline__ void sum_runs(const Segments& S, const uint32_t* skey, int len, bool col_ok,
-                                         RunShared<V>& sh, F load, W write, H write_head, L write_tail) {
+                                         RunShared<V, THREADS>& sh, F load, W write, H write_head, L write_tail) {
     typedef typename VecOf<T, V>::type vec;
-    const int lanes = 1 << S.lg, n_groups = 256 >> S.lg;
+    const int lanes = 1 << S.lg, n_groups = THREADS >> S.lg;
     const int g = threadIdx.x >> S.lg;
     const int first = min(g * S.per_group, len), last = min(first + S.per_group, len);
     float acc[V], head[V];
@@ -418,7 +419,7 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const uint32_t* skey
     bool open = has_tail && from_left;
     const int l = threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < V; ++k) sh.val[k * 256 + l] = acc[k];
+    for (int k = 0; k < V; ++k) sh.val[k * THREADS + l] = acc[k];
     sh.open[l] = open;
     for (int s = 1; s < n_groups; s <<= 1) {
         const int q = l - (s << S.lg);
@@ -429,12 +430,12 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const uint32_t* skey
         if (add) {
             o = sh.open[q];
 #pragma unroll
-            for (int k = 0; k < V; ++k) t[k] = sh.val[k * 256 + q];
+            for (int k = 0; k < V; ++k) t[k] = sh.val[k * THREADS + q];
         }
         __syncthreads();
         if (add) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) sh.val[k * 256 + l] = acc[k] = t[k] + acc[k];
+            for (int k = 0; k < V; ++k) sh.val[k * THREADS + l] = acc[k] = t[k] + acc[k];
             sh.open[l] = open = o;
         }
     }
@@ -446,7 +447,7 @@ __device__ __forceinline__ void sum_runs(const Segments& S, const uint32_t* skey
             const int q = l - lanes;
             before_piece = sh.open[q];
 #pragma unroll
-            for (int k = 0; k < V; ++k) head[k] += sh.val[k * 256 + q];
+            for (int k = 0; k < V; ++k) head[k] += sh.val[k * THREADS + q];
         }
         if (col_ok) {
             if (before_piece) write_head(head); else write(head_key, head);
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* _
                                                           O* __restrict__ out) {
     typedef typename VecOf<T, V>::type vec;
     extern __shared__ uint32_t smem[];                // (the usual piece takes a few hundred bytes)
-    __shared__ RunShared<V> sh;
+    __shared__ RunShared<V, 256> sh;
     const int lanes = 1 << S.lg;
     const int64_t j = (int64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
     const bool col_ok = j * V < S.D;
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(256) void row_segment_kernel(Segments S, const T* _
     char* to = reinterpret_cast<char*>(out + c);
     const uint32_t pitch = (uint32_t)S.ld * sizeof(T), out_pitch = (uint32_t)S.D * sizeof(O);
     uint8_t* touched = j == 0 ? S.touched : nullptr;
-    sum_runs<T, V>(
+    sum_runs<T, V, 256>(
         S, skey, len, col_ok, sh,
         [&](int i) { return *reinterpret_cast<const vec*>(from + row_offset(spos[i], pitch)); },
         [&](uint32_t row, const float* f) {
@@ -572,15 +573,15 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
 // are the rows themselves; otherwise row r of tile t goes to partial[r][t], met[r][t] says
 // whether the tile has it.
 template <typename T, typename O, typename I, int V, bool ALONE>
-__global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __restrict__ grad,
+__global__ __launch_bounds__(kTileThreads) void row_tile_kernel(Segments S, const T* __restrict__ grad,
                                                        const I* __restrict__ ids, IdRange range, int bits,
                                                        O* __restrict__ out, uint8_t* __restrict__ met,
                                                        int keep_touched) {
-    __shared__ uint16_t counts[4][kRadix];
+    __shared__ uint16_t counts[kTileThreads / 64][kRadix];
     __shared__ uint32_t base[kRadix + 1], wsum[4];
     __shared__ uint32_t skey[kTileIds + 2];
     __shared__ uint32_t spos[kTileIds];               // byte offsets of the rows inside the tile
-    __shared__ RunShared<V> sh;
+    __shared__ RunShared<V, kTileThreads> sh;
     typedef typename VecOf<T, V>::type vec;
     const uint32_t pitch = (uint32_t)S.ld * sizeof(T);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
         const int i = (w * kTileItems + r) * 64 + lane;
         key[r] = sort_key(ids[first + min(i, len - 1)], range);
     }
-    block_digit_places<4, kTileItems>(key, len, 0, bits, counts, base, wsum, place);
+    block_digit_places<kTileThreads / 64, kTileItems>(key, len, 0, bits, counts, base, wsum, place);
 #pragma unroll
     for (int r = 0; r < kTileItems; ++r) {
         const int i = (w * kTileItems + r) * 64 + lane;
@@ -601,7 +602,7 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
     if (threadIdx.x == 0) { skey[0] = skey[len + 1] = kNoKey; base[kRadix] = (uint32_t)len; }
     __syncthreads();
     const int64_t tiles = gridDim.x;
-    for (uint32_t r = threadIdx.x; r < S.rows; r += 256) {
+    for (uint32_t r = threadIdx.x; r < S.rows; r += kTileThreads) {
         const uint8_t any = base[r + 1] > base[r];
         if (!ALONE) met[r * tiles + blockIdx.x] = any;
         else if (S.touched && (any || !keep_touched)) S.touched[r] = any;
@@ -612,7 +613,7 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
     const int64_t c = col_ok ? vec_col<V>(j, S.D) : 0;
     if (ALONE && col_ok) {
         const float zero[V] = {};
-        for (uint32_t r = threadIdx.x >> S.lg; r < S.rows; r += 256 >> S.lg)
+        for (uint32_t r = threadIdx.x >> S.lg; r < S.rows; r += kTileThreads >> S.lg)
             if (base[r + 1] == base[r]) store_cols<O, V>(out + (int64_t)r * S.D + c, zero);
     }
     const char* from = reinterpret_cast<const char*>(grad + first * S.ld + c);
@@ -620,7 +621,7 @@ __global__ __launch_bounds__(256) void row_tile_kernel(Segments S, const T* __re
     char* to = ALONE ? reinterpret_cast<char*>(out + c)
                      : reinterpret_cast<char*>(S.partial + blockIdx.x * S.D + c);
     const uint32_t out_pitch = ALONE ? (uint32_t)S.D * sizeof(O) : (uint32_t)(tiles * S.D) * 4u;
-    sum_runs<T, V>(
+    sum_runs<T, V, kTileThreads>(
         S, skey, len, col_ok, sh, [&](int i) { return *reinterpret_cast<const vec*>(from + spos[i]); },
         [&](uint32_t row, const float* f) {
             char* q = to + row_offset(row, out_pitch);
@@ -702,14 +703,15 @@ SegmentPlan plan_segments(int64_t N, int64_t rows, int64_t D, int type) {
     const int64_t vectors = (D + p.vec - 1) / p.vec;
     p.lg = vectors >= 64 ? 6 : ceil_log2(vectors);
     p.segments = (int)((vectors + (1 << p.lg) - 1) >> p.lg);
-    const int groups = 256 >> p.lg;
     // few rows: one digit, a lane group of the tile sums at most 64 positions
     p.few = rows <= kFewRows && vectors <= 16 && N <= (int64_t)kFewTiles * kTileIds;
     if (p.few) {
+        const int groups = kTileThreads >> p.lg;
         p.per_group = (int)((std::min<int64_t>(N, kTileIds) + groups - 1) / groups);
         p.pieces = (int)((N + kTileIds - 1) / kTileIds);
         return p;
     }
+    const int groups = 256 >> p.lg;
     // about 2048 workgroups (eight per CU) where there are enough ids; 4 positions at least (the
     // loads a lane keeps in flight), 64 at most (what one float32 sum may run over)
     const int64_t per = N * p.segments / ((int64_t)groups * 2048);
@@ -824,10 +826,10 @@ template <typename T, typename O, typename I, int V>
 int few_launches(const Segments& S, const SegmentPlan& p, const GradWorkspace& w, const void* grad, const void* ids,
                  IdRange range, int bits, void* out, int keep_touched, hipStream_t s) {
     if (p.pieces == 1)
-        row_tile_kernel<T, O, I, V, true><<<1, 256, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out, w.met,
+        row_tile_kernel<T, O, I, V, true><<<1, kTileThreads, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out, w.met,
                                                             keep_touched);
     else
-        row_tile_kernel<T, O, I, V, false><<<p.pieces, 256, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out,
+        row_tile_kernel<T, O, I, V, false><<<p.pieces, kTileThreads, 0, s>>>(S, (const T*)grad, (const I*)ids, range, bits, (O*)out,
                                                                     w.met, keep_touched);
     VINGS_LAUNCH_CHECK();
     if (p.pieces > 1) {

@@ -430,7 +430,7 @@ def test_backward_arguments():
     assert call(rows=0, out=None) == 0
     for change, text in ((dict(n=-1), "sizes"), (dict(cols=0), "sizes"), (dict(ot=1), "gradient's type"), (dict(ty=1, ot=2), "gradient's type"),
                          (dict(out=None), "null pointer"), (dict(grad=None), "null pointer"), (dict(ids=None), "null pointer"),
-                         (dict(ws=None), "null pointer"), (dict(ld=-1), "sizes"), (dict(ws=FAKE + 8), "256-byte"),
+                         (dict(ws=None), "null pointer"), (dict(ld=-1), "2^22"), (dict(ld=2 ** 22), "2^22"), (dict(ws=FAKE + 8), "256-byte"),
                          (dict(ws_bytes=16), "too small"), (dict(out=FAKE + 2), "alignment"), (dict(grad=FAKE + 1), "alignment")):
         assert call(**change) != 0 and text in _error(), change
     assert size(0, 9, 4, 0) == 0 and size(10, 9, 4, 9) == 0 and size(10, 0, 4, 0) == 0

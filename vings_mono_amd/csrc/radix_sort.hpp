@@ -123,6 +123,21 @@ static __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
     __shared__ uint32_t lkey[kSortTile];
     __shared__ uint32_t lval[kSortTile];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t wbase = (int64_t)blockIdx.x * kSortTile + w * (kSortItems * 64);
+    uint32_t key[kSortItems];
+    uint32_t val[kSortItems];
+    uint32_t rank[kSortItems];
+    // (unguarded loads, see above, under way while the digit bases are formed; a speculative
+    // launch may have tiles behind the last key)
+    if ((int64_t)blockIdx.x * kSortTile < D) {
+#pragma unroll
+        for (int r = 0; r < kSortItems; ++r) {
+            const int64_t i = wbase + r * 64 + lane, at = min(i, D - 1);
+            key[r] = sort_key(keys_in[at], range);
+            if constexpr (kIds<K>) val[r] = (uint32_t)i;
+            else val[r] = vals_in[at];
+        }
+    }
     for (int k = threadIdx.x; k < 4 * kRadix; k += kSortThreads) (&wcount[0][0])[k] = 0;
     // first output slot of digit d in this tile = keys with a smaller digit anywhere
     // (exclusive prefix of the 256 digit totals, one digit per lane) + keys with digit d in
@@ -136,21 +151,9 @@ static __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
     gbase[threadIdx.x] = below + thist[(size_t)threadIdx.x * ntiles + blockIdx.x];
     __syncthreads();
 
-    const int64_t wbase = (int64_t)blockIdx.x * kSortTile + w * (kSortItems * 64);
-    uint32_t key[kSortItems];
-    uint32_t val[kSortItems];
-    uint32_t rank[kSortItems];
     const uint64_t lt_mask = lane == 0 ? 0ull : (~0ull >> (64 - lane));
-    // (unguarded loads, see above; a speculative launch may have tiles behind the last key)
-    if ((int64_t)blockIdx.x * kSortTile < D) {
-#pragma unroll
-        for (int r = 0; r < kSortItems; ++r) {
-            const int64_t i = wbase + r * 64 + lane, at = min(i, D - 1);
-            key[r] = sort_key(keys_in[at], range);
-            if constexpr (kIds<K>) val[r] = (uint32_t)i;
-            else val[r] = vals_in[at];
-        }
-    }
+    // which lanes hold the same digit: independent for the rounds, so their ballots overlap
+    uint32_t peers_n[kSortItems];
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
         const bool valid = wbase + r * 64 + lane < D;
@@ -165,11 +168,18 @@ static __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
             }
         }
         // all lanes in `peers` share digit d (invalid lanes excluded)
+        rank[r] = __popcll(peers & lt_mask);
+        peers_n[r] = valid ? __popcll(peers) : 0u;
+    }
+    // ... then the chain of per-wave digit counters
+#pragma unroll
+    for (int r = 0; r < kSortItems; ++r) {
+        const uint32_t d = digit_of(key[r], shift);
         const uint32_t before = wcount[w][d];  // read before the leader updates it
-        const uint32_t below = __popcll(peers & lt_mask);
-        rank[r] = before + below;
+        const bool leader = peers_n[r] && rank[r] == 0;
+        rank[r] += before;
         __builtin_amdgcn_wave_barrier();
-        if (valid && below == 0) wcount[w][d] = before + __popcll(peers);
+        if (leader) wcount[w][d] = before + peers_n[r];
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();

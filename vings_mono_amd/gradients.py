@@ -9,7 +9,8 @@ writing them, pass `max_norm` to `surfel.SparseGaussianAdam.step`.
 Everything stays on the device and on the current stream: nothing synchronises (except
 `error_if_nonfinite`), so the calls can be captured into a graph.
 """
-import ctypes
+import array
+import operator
 
 import torch
 
@@ -19,10 +20,15 @@ from ._lib import VingsError, check, stream_ptr
 _KINDS = {2.0: 0, float("inf"): 1}
 
 
+# (lists of hundreds of small tensors are bound by the host: a bound method mapped over the list
+# costs a third of the same attribute in a loop)
+_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
+_get_device, _is_contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+_dtype = operator.attrgetter("dtype")
+
+
 def _dense(t):
     """Whether the elements of t fill one stretch of memory, in whatever order of dimensions."""
-    if t.is_contiguous():
-        return True
     expected = 1
     for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: d[1]):
         if size == 1:
@@ -33,23 +39,43 @@ def _dense(t):
     return True
 
 
-def _checked(tensors, what):
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not tensors:
-        raise VingsError(f"{what}: no tensors given")
-    dev = tensors[0].device
-    for t in tensors:
-        _lib.require_gpu_tensor(t, what)
-        if t.layout != torch.strided:
-            raise VingsError(f"{what}: sparse tensors are not supported")
-        if t.dtype not in _lib.ELEM_TYPES:
-            raise VingsError(f"{what}: float32, bfloat16 or float16 expected (got {t.dtype})")
-        if t.device != dev:
-            raise VingsError(f"{what}: all tensors must live on one device ({dev} and {t.device})")
-        if not _dense(t):
-            raise VingsError(f"{what}: a tensor with gaps or overlaps between its elements "
-                             f"(shape {tuple(t.shape)}, strides {t.stride()}); pass a contiguous copy")
-    return tensors, dev
+class _List:
+    """A checked list of tensors and the tables the C entry points take."""
+    __slots__ = ("tensors", "device", "contiguous", "n", "numels", "pointers", "types")
+
+    def __init__(self, tensors, what):
+        self.tensors = tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        if not tensors:
+            raise VingsError(f"{what}: no tensors given")
+        self.device = tensors[0].device
+        types = list(map(_lib.ELEM_TYPES.get, map(_dtype, tensors)))
+        if None in types or set(map(_get_device, tensors)) != {self.device.index}:
+            self._refuse(what)
+        try:
+            self.contiguous = all(map(_is_contiguous, tensors))
+            pointers = array.array("Q", map(_data_ptr, tensors))
+        except RuntimeError:
+            raise VingsError(f"{what}: sparse tensors are not supported") from None
+        if not self.contiguous:
+            for t in tensors:
+                if not t.is_contiguous() and not _dense(t):
+                    raise VingsError(f"{what}: a tensor with gaps or overlaps between its elements "
+                                     f"(shape {tuple(t.shape)}, strides {t.stride()}); pass a contiguous copy")
+        self.n = len(tensors)
+        self.pointers, self.types = pointers, array.array("i", types)
+        self.numels = array.array("q", map(_numel, tensors))
+
+    def _refuse(self, what):
+        for t in self.tensors:
+            _lib.require_gpu_tensor(t, what)
+            if t.dtype not in _lib.ELEM_TYPES:
+                raise VingsError(f"{what}: float32, bfloat16 or float16 expected (got {t.dtype})")
+            if t.device != self.device:
+                raise VingsError(f"{what}: all tensors must live on one device ({self.device} and {t.device})")
+
+
+def _address(table):
+    return table.buffer_info()[0]
 
 
 def _kind(norm_type):
@@ -57,14 +83,6 @@ def _kind(norm_type):
     if kind is None:
         raise VingsError(f"norm_type must be 2 or inf (got {norm_type})")
     return kind
-
-
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
-
-
-def _types(tensors):
-    return (ctypes.c_int * len(tensors))(*[_lib.ELEM_TYPES[t.dtype] for t in tensors])
 
 
 def norm_and_workspace(nbytes, dev):
@@ -81,14 +99,13 @@ def global_norm(tensors, norm_type=2.0):
     norm_type=inf.  Sums are held in 64 bits: no overflow below the largest float32 norm.  A
     tensor given twice counts twice."""
     kind = _kind(norm_type)
-    tensors, dev = _checked(tensors, "global_norm")
-    L, n = _lib.lib(), len(tensors)
-    numels = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    with _lib.on_device(dev):
-        nbytes = L.vings_grad_norm_workspace_bytes(n, numels)
-        norm, ws = norm_and_workspace(nbytes, dev)
-        check(L.vings_grad_norm(n, _pointers(tensors), numels, _types(tensors), kind, norm.data_ptr(),
-                                ws, nbytes, stream_ptr(dev)), "vings_grad_norm")
+    g = _List(tensors, "global_norm")
+    L, numels = _lib.lib(), _address(g.numels)
+    with _lib.on_device(g.device):
+        nbytes = L.vings_grad_norm_workspace_bytes(g.n, numels)
+        norm, ws = norm_and_workspace(nbytes, g.device)
+        check(L.vings_grad_norm(g.n, _address(g.pointers), numels, _address(g.types), kind, norm.data_ptr(),
+                                ws, nbytes, stream_ptr(g.device)), "vings_grad_norm")
     return norm
 
 
@@ -103,28 +120,25 @@ def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
-    tensors, dev = _checked(tensors, "clip_by_global_norm")
-    if out is None:
-        outs = tensors
-    else:
-        outs, out_dev = _checked(out, "clip_by_global_norm: out")
-        if len(outs) != len(tensors) or out_dev != dev:
+    g = _List(tensors, "clip_by_global_norm")
+    o = g
+    if out is not None:
+        o = _List(out, "clip_by_global_norm: out")
+        if o.n != g.n or o.device != g.device:
             raise VingsError("out must hold one tensor per gradient, on the gradients' device")
-        for t, o in zip(tensors, outs):
-            if t.shape != o.shape or (t.stride() != o.stride() and not (t.is_contiguous() and o.is_contiguous())):
+        for t, u in zip(g.tensors, o.tensors):
+            if t.shape != u.shape or (t.stride() != u.stride() and not (t.is_contiguous() and u.is_contiguous())):
                 raise VingsError("out must have the shapes and strides of the gradients")
-            if o.dtype not in (t.dtype, torch.float32):
-                raise VingsError(f"a clipped {t.dtype} gradient is {t.dtype} or float32 (got {o.dtype})")
-    L, n = _lib.lib(), len(tensors)
-    numels = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    ins, types = _pointers(tensors), _types(tensors)
-    with _lib.on_device(dev):
-        nbytes = L.vings_grad_norm_workspace_bytes(n, numels)
-        norm, ws = norm_and_workspace(nbytes, dev)
-        check(L.vings_grad_clip(n, ins, ins if out is None else _pointers(outs), numels, types,
-                                types if out is None else _types(outs), kind, max_norm, norm.data_ptr(),
-                                ws, nbytes, stream_ptr(dev)), "vings_grad_clip")
-    torch.autograd.graph.increment_version(outs)
+            if u.dtype not in (t.dtype, torch.float32):
+                raise VingsError(f"a clipped {t.dtype} gradient is {t.dtype} or float32 (got {u.dtype})")
+    L, numels = _lib.lib(), _address(g.numels)
+    with _lib.on_device(g.device):
+        nbytes = L.vings_grad_norm_workspace_bytes(g.n, numels)
+        norm, ws = norm_and_workspace(nbytes, g.device)
+        check(L.vings_grad_clip(g.n, _address(g.pointers), _address(o.pointers), numels, _address(g.types),
+                                _address(o.types), kind, max_norm, norm.data_ptr(), ws, nbytes,
+                                stream_ptr(g.device)), "vings_grad_clip")
+    torch.autograd.graph.increment_version(o.tensors)
     return norm
 
 

@@ -7,6 +7,7 @@ imports at /root/reference/scripts/gaussian/gaussian_base.py:5-6:
 ABI of include/vings_hip.h; torch only provides device memory, the current
 stream and the autograd hook.
 """
+import array
 import ctypes
 import os
 from typing import NamedTuple, Optional
@@ -625,15 +626,15 @@ class SparseGaussianAdam(torch.optim.Adam):
         n = len(consts)
         if n == 0:
             return torch.zeros((), dtype=torch.float32, device=dev)
-        col = lambda k, kind: (kind * n)(*[c[k] for c in consts])
-        tables = [(ctypes.c_void_p * n)(*arrays[k::4]) for k in range(4)]
+        widths, lrs, b1s, b2s, epss = zip(*consts)
+        tables = [array.array("Q", arrays[k::4]) for k in range(4)]
+        tables += [array.array("i", widths), array.array("f", lrs), array.array("d", b1s), array.array("d", b2s),
+                   array.array("f", epss)]
         with _lib.on_device(dev):
             nbytes = L.vings_sparse_adam_clipped_workspace_bytes(n)
             norm, ws = norm_and_workspace(nbytes, dev)
             check(L.vings_sparse_adam_clipped(
-                n, *tables, col(0, ctypes.c_int), col(1, ctypes.c_float), col(2, ctypes.c_double),
-                col(3, ctypes.c_double), col(4, ctypes.c_float),
-                ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
+                n, *[t.buffer_info()[0] for t in tables], ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
                 None if guard is None else guard[0], 0 if guard is None else int(guard[1]),
                 stream_ptr(dev)), "vings_sparse_adam_clipped")
         return norm

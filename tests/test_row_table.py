@@ -102,7 +102,9 @@ def test_lookup(n, rows, cols, dtype):
 @gpu
 @pytest.mark.parametrize("how", ["uniform", "one", "power", "sorted", "none", "strays"])
 @pytest.mark.parametrize("n,rows,cols", SHAPES + [(16385, 70000, 8), (50001, 300, 9), (200003, 80, 12), (70000, 3, 2),
-                                                  (20000, 5, 640), (30000, 60000, 20)])
+                                                  (20000, 5, 640), (30000, 60000, 20), (3000, 255, 4), (3000, 256, 4),
+                                                  (90001, 1999, 64), (1024, 4095, 16), (1025, 4095, 3), (5000, 4096, 16),
+                                                  (40000, 257, 60), (2600, 700, 68)])
 def test_backward(n, rows, cols, how):
     dtype = TYPES[(n + cols) % 3]
     id_type = (torch.int64, torch.int32)[(n + rows) % 2]
@@ -425,7 +427,7 @@ def test_backward_arguments():
     L = _lib.lib()
     size = L.vings_row_lookup_backward_workspace_bytes
 
-    def call(n=4, rows=500, cols=3, grad=FAKE, ld=3, ty=0, ids=FAKE, idb=8, out=FAKE, ot=0, ws=FAKE, ws_bytes=1 << 20):
+    def call(n=4, rows=5000, cols=3, grad=FAKE, ld=3, ty=0, ids=FAKE, idb=8, out=FAKE, ot=0, ws=FAKE, ws_bytes=1 << 20):
         return L.vings_row_lookup_backward(n, rows, cols, grad, ld, ty, ids, idb, -1, 1.0, out, ot, None, 0, ws, ws_bytes, None)
     assert call(rows=0, out=None) == 0
     for change, text in ((dict(n=-1), "sizes"), (dict(cols=0), "sizes"), (dict(ot=1), "gradient's type"), (dict(ty=1, ot=2), "gradient's type"),
@@ -434,4 +436,4 @@ def test_backward_arguments():
                          (dict(ws_bytes=16), "too small"), (dict(out=FAKE + 2), "alignment"), (dict(grad=FAKE + 1), "alignment")):
         assert call(**change) != 0 and text in _error(), change
     assert size(0, 9, 4, 0) == 0 and size(10, 9, 4, 9) == 0 and size(10, 0, 4, 0) == 0
-    assert size(10, 300, 4, 0) >= 80 and size(100000, 300, 4, 0) >= 4 * 4 * 100000     # both sides of the passes
+    assert size(10, 5000, 4, 0) >= 80 and size(100000, 5000, 4, 0) >= 4 * 4 * 100000   # both sides of the passes

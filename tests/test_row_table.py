@@ -104,7 +104,8 @@ def test_lookup(n, rows, cols, dtype):
 @pytest.mark.parametrize("n,rows,cols", SHAPES + [(16385, 70000, 8), (50001, 300, 9), (200003, 80, 12), (70000, 3, 2),
                                                   (20000, 5, 640), (30000, 60000, 20), (3000, 255, 4), (3000, 256, 4),
                                                   (90001, 1999, 64), (1024, 4095, 16), (1025, 4095, 3), (5000, 4096, 16),
-                                                  (40000, 257, 60), (2600, 700, 68)])
+                                                  (40000, 257, 60), (2600, 700, 68), (32768, 5000, 12),
+                                                  (32769, 5000, 12), (9000, 70000, 24), (17000, 4097, 300)])
 def test_backward(n, rows, cols, how):
     dtype = TYPES[(n + cols) % 3]
     id_type = (torch.int64, torch.int32)[(n + rows) % 2]

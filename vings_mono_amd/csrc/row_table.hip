@@ -8,7 +8,7 @@
 //
 // The gradient sums by SORTED ids, with no float atomics, so its bits do not depend on timing:
 //   1. the ids and their positions are ordered by a stable radix sort; ids that name no row sort
-//      behind the last row.  Up to 16384 ids workgroups sort runs of 1024 in LDS and a second
+//      behind the last row.  Up to 32768 ids workgroups sort runs of 1024 in LDS and a second
 //      launch merges the runs, every id finding its place by bisection in each of them, while
 //      further workgroups of both launches clear dtable and touched; more ids take the tile
 //      passes of radix_sort.hpp, 8 bits each
@@ -39,7 +39,7 @@
 namespace vings {
 
 constexpr int kRun = 1024;                // ids a workgroup sorts in LDS
-constexpr int kMaxRuns = 16;              // runs the merge launch takes
+constexpr int kMaxRuns = 32;              // runs the merge launch takes
 constexpr int kMergeSortMax = kRun * kMaxRuns;
 constexpr int kTileThreads = 512;         // few-rows form: lanes and
 constexpr int kTileIds = 1024;            // ids per workgroup
@@ -272,27 +272,29 @@ __global__ __launch_bounds__(1024) void row_sort_runs_kernel(const I* __restrict
 // Merges up to kMaxRuns sorted runs: the place of an id is its place in its own run plus, for
 // every earlier run, the ids there that are not larger, and for every later one those that are
 // smaller.  All keys sit in LDS; four bisections of a lane run side by side.
+// (RUNS: the LDS that the launch reserves, for its clearing workgroups too.)
 constexpr int kMergeThreads = 256;
+template <int RUNS>
 __global__ __launch_bounds__(kMergeThreads) void row_merge_runs_kernel(
     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int N, int n_runs, int n_merge,
     uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out, Fill F) {
-    __shared__ __align__(16) uint32_t lkey[kMergeSortMax];
+    __shared__ __align__(16) uint32_t lkey[RUNS * kRun];
     if ((int)blockIdx.x >= n_merge) {
         clear(F, (int64_t)(blockIdx.x - n_merge) * kMergeThreads + threadIdx.x,
               (int64_t)(gridDim.x - n_merge) * kMergeThreads);
         return;
     }
     // (all loads in flight together: the launch is a chain of latencies)
-    uint4 q[kMaxRuns];
+    uint4 q[RUNS];
     static_assert(kRun == 4 * kMergeThreads, "a run is one round of 16-byte loads");
 #pragma unroll
-    for (int r = 0; r < kMaxRuns; ++r) {
+    for (int r = 0; r < RUNS; ++r) {
         // (a load that begins before N ends inside the array's 256-byte granule)
         const int i = r * kRun + 4 * threadIdx.x;
         q[r] = *reinterpret_cast<const uint4*>(keys + (i < N ? i : 0));
     }
 #pragma unroll
-    for (int r = 0; r < kMaxRuns; ++r) {
+    for (int r = 0; r < RUNS; ++r) {
         const int i = r * kRun + 4 * threadIdx.x;
         const uint4 k = make_uint4(i < N ? q[r].x : ~0u, i + 1 < N ? q[r].y : ~0u, i + 2 < N ? q[r].z : ~0u,
                                    i + 3 < N ? q[r].w : ~0u);
@@ -827,13 +829,13 @@ int sort_runs(const I* ids, int N, IdRange range, int bits, const GradWorkspace&
               hipStream_t s) {
     const int runs = cdiv(N, kRun);
     // clearing in 64 KB per workgroup, four per CU at most; three quarters beside the first
-    // launch, which leaves more of every CU free
+    // launch, which leaves more of every CU free, all of it where the merge takes most of the LDS
     auto blocks = [](const Fill& f) {
         return (int)std::min<int64_t>(1024, (f.bytes + f.n_touched + 65535) / 65536);
     };
     Fill A = F, B = F;
     if (runs > 1) {
-        A.bytes = (F.bytes / 4 * 3) & ~(int64_t)15;
+        A.bytes = runs > 16 ? F.bytes : (F.bytes / 4 * 3) & ~(int64_t)15;
         A.n_touched = 0;
         B.rows = (char*)F.rows + A.bytes;
         B.bytes = F.bytes - A.bytes;
@@ -843,8 +845,12 @@ int sort_runs(const I* ids, int N, IdRange range, int bits, const GradWorkspace&
     *at = 0;
     if (runs == 1) return VINGS_OK;
     const int merge = cdiv(N, kMergeThreads);
-    row_merge_runs_kernel<<<merge + blocks(B), kMergeThreads, 0, s>>>(w.key[0], w.val[0], N, runs, merge,
-                                                                      w.key[1], w.val[1], B);
+    auto launch = [&](auto kernel) {
+        kernel<<<merge + blocks(B), kMergeThreads, 0, s>>>(w.key[0], w.val[0], N, runs, merge, w.key[1], w.val[1], B);
+    };
+    if (runs <= 8) launch(row_merge_runs_kernel<8>);
+    else if (runs <= 16) launch(row_merge_runs_kernel<16>);
+    else launch(row_merge_runs_kernel<32>);
     VINGS_LAUNCH_CHECK();
     *at = 1;
     return VINGS_OK;

@@ -176,11 +176,14 @@ def stream_ptr(device=None):
 ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # VINGS_F32, _BF16, _F16
 
 
+_CURRENT = contextlib.nullcontext()
+
+
 def on_device(device):
     """Context in which kernels are launched for tensors of `device`: that device is made current
     for the call if it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _CURRENT
     return torch.cuda.device(device)
 
 

@@ -12,10 +12,15 @@ from . import _lib
 from ._lib import VingsError, check, stream_ptr
 
 
-def _rows_2d(t, name):
+_ID_TYPES = (torch.int32, torch.int64)
+
+
+def _rows_2d(t):
     """t [..., D] as rows with unit column stride: (tensor, number of rows, row stride)."""
     D = t.shape[-1]
-    n = t.numel() // D if D else 0
+    n = t.numel() // D
+    if t.is_contiguous():
+        return t, n, D
     if t.dim() == 2 and (t.stride(1) == 1 or D == 1) and (n <= 1 or D <= t.stride(0) < 1 << 22 or t.stride(0) == 0):
         return t, n, t.stride(0) if n > 1 else D
     t = t.contiguous()
@@ -23,13 +28,13 @@ def _rows_2d(t, name):
 
 
 def _check(t, ids, name):
-    _lib.require_gpu_tensor(t, name)
-    _lib.require_gpu_tensor(ids, "ids")
-    if t.device != ids.device:
+    if t.get_device() != ids.get_device() or t.get_device() < 0:
+        _lib.require_gpu_tensor(t, name)
+        _lib.require_gpu_tensor(ids, "ids")
         raise VingsError(f"{name} and ids must live on one device ({t.device} and {ids.device})")
     if t.dtype not in _lib.ELEM_TYPES:
         raise VingsError(f"{name}: float32, bfloat16 or float16 expected (got {t.dtype})")
-    if ids.dtype not in (torch.int32, torch.int64):
+    if ids.dtype not in _ID_TYPES:
         raise VingsError(f"ids must be int32 or int64 (got {ids.dtype})")
     if t.dim() < 1 or t.shape[-1] == 0:
         raise VingsError(f"{name} must have at least one column (got shape {tuple(t.shape)})")
@@ -45,21 +50,22 @@ def _check_touched(touched, num_rows, device):
 
 def _lookup(table, ids, scale):
     V, D = table.shape
-    src, _, ld = _rows_2d(table, "table")
+    src, _, ld = _rows_2d(table)
     if ld == 0:
         src, ld = table.contiguous(), D
     flat = ids.contiguous()
-    out = torch.empty(tuple(ids.shape) + (D,), dtype=table.dtype, device=table.device)
-    with _lib.on_device(table.device):
+    dev, dtype = table.device, table.dtype
+    out = torch.empty((*ids.shape, D), dtype=dtype, device=dev)
+    with _lib.on_device(dev):
         check(_lib.lib().vings_row_lookup(
-            flat.numel(), V, D, src.data_ptr(), ld, _lib.ELEM_TYPES[table.dtype], flat.data_ptr(),
-            flat.element_size(), scale, out.data_ptr(), stream_ptr(table.device)), "vings_row_lookup")
+            flat.numel(), V, D, src.data_ptr(), ld, _lib.ELEM_TYPES[dtype], flat.data_ptr(),
+            flat.element_size(), scale, out.data_ptr(), stream_ptr(dev)), "vings_row_lookup")
     return out
 
 
 def _lookup_backward(grad, ids, num_rows, scale, padding_id, out, touched, keep_touched):
     D = grad.shape[-1]
-    src, n, ld = _rows_2d(grad, "grad")
+    src, n, ld = _rows_2d(grad)
     flat = ids.contiguous()
     L, dev, et = _lib.lib(), grad.device, _lib.ELEM_TYPES[grad.dtype]
     with _lib.on_device(dev):

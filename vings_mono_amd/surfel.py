@@ -595,7 +595,7 @@ class SparseGaussianAdam(torch.optim.Adam):
     def _clipped_step(self, L, vis, N, guard, max_norm):
         if not max_norm >= 0.0:
             raise _lib.VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
-        dev = vis.device
+        dev, index = vis.device, vis.get_device()
         arrays, keep, consts = [], [], []
         for group in self.param_groups:
             if len(group["params"]) != 1:
@@ -605,7 +605,7 @@ class SparseGaussianAdam(torch.optim.Adam):
             if g is None:
                 continue
             _lib.require_gpu_tensor(p, "param", torch.float32)
-            if p.device != dev or g.device != dev:
+            if p.get_device() != index or g.get_device() != index:
                 raise _lib.VingsError("parameters, gradients and visibility must live on one device")
             if g.dtype != torch.float32:
                 raise _lib.VingsError(f"gradients must be float32 (got {g.dtype})")
@@ -615,12 +615,11 @@ class SparseGaussianAdam(torch.optim.Adam):
             if size % N != 0:
                 raise _lib.VingsError("parameter size is not a multiple of N")
             state = self._moments(p)
-            g = g.contiguous()
-            keep.append(g)
-            for t in (p, g, state["exp_avg"], state["exp_avg_sq"]):
-                if not t.is_contiguous() or t.numel() != size:
-                    raise _lib.VingsError("parameters and moments must be dense and of one size")
-                arrays.append(t.data_ptr())
+            quad = (p, g.contiguous(), state["exp_avg"], state["exp_avg_sq"])
+            keep.append(quad)
+            if not all([t.is_contiguous() and t.numel() == size for t in quad]):
+                raise _lib.VingsError("parameters and moments must be dense and of one size")
+            arrays += [t.data_ptr() for t in quad]
             b1, b2 = group.get("betas", (0.9, 0.999))
             consts.append((size // N, group["lr"], b1, b2, group["eps"]))
         n = len(consts)

@@ -295,7 +295,8 @@ int vings_grad_clip(int n_tensors, const void* const* grads_host, void* const* o
  * gradient's type or VINGS_F32.  ids int32 or int64 (id_bytes).  Sums are float32, in an order
  * fixed by the ids alone, rounded once.  touched (may be NULL) [n_rows]: 1 for rows that some id
  * names, else 0 -- or left as it is with keep_touched, so that several calls can mark one array.
- * Sizes: n_ids, n_rows < 2^31 - 1, 0 < n_cols < 2^22, grad_stride < 2^22. */
+ * Sizes: n_ids, n_rows < 2^31 - 1, 0 < n_cols <= 2^20, grad_stride <= 2^20.  rows and touched
+ * overlap no other array of the call. */
 int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, const void* table,
                      int64_t table_stride, int type, const void* ids, int id_bytes, float scale,
                      void* out, void* stream);

@@ -200,6 +200,21 @@ def test_strided_rows_and_unaligned_views(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [40, 3000, 5000])
+@pytest.mark.parametrize("stride", [1 << 20, (1 << 20) + 8])
+def test_gradient_rows_far_apart(rows, stride):
+    """The largest row distance that is read where it lies, and one that is copied first: byte
+    offsets inside a tile of 1024 rows reach 2^32 there."""
+    n = 1100
+    far = torch.zeros(n * stride, device=DEV)
+    grad = far.as_strided((n, 5), (stride, 1))
+    grad.copy_(rand((n, 5), seed=2))
+    ids = make_ids(n, rows, "uniform")
+    got, touched = row_table.lookup_rows_backward(grad, ids, rows)
+    check_backward(grad.contiguous(), ids, rows, 1.0, got, touched)
+
+
+@gpu
 def test_what_stands_behind_unused_ids_is_not_read():
     """Gradient rows of ids that name no row may hold anything."""
     grad = rand((500, 16), seed=1)
@@ -284,6 +299,7 @@ def test_refusals_on_the_device():
                  lambda: row_table.lookup_rows_backward(g, ids, 5, out=torch.empty((5, 3), device=DEV)),
                  lambda: row_table.lookup_rows_backward(g, ids, 5, out=torch.empty((5, 4), dtype=torch.bfloat16, device=DEV)),
                  lambda: row_table.lookup_rows_backward(g, ids, 5, out=torch.empty((4, 5), device=DEV).t()),
+                 lambda: row_table.lookup_rows_backward(t[:3], ids, 5, out=t),
                  lambda: row_table.lookup_rows_backward(g, ids, 2 ** 31)):
         with pytest.raises(_lib.VingsError):
             call()
@@ -416,7 +432,7 @@ def test_lookup_arguments():
         return _lib.lib().vings_row_lookup(n, rows, cols, table, ld, ty, ids, idb, 1.0, out, None)
     assert call(n=0, table=None, ids=None, out=None) == 0
     for change, text in ((dict(n=-1), "sizes"), (dict(rows=-1), "sizes"), (dict(cols=0), "sizes"), (dict(rows=2 ** 31), "31 bits"),
-                         (dict(n=2 ** 31), "31 bits"), (dict(cols=2 ** 22), "22"), (dict(ty=3), "element type"), (dict(ty=-1), "element type"),
+                         (dict(n=2 ** 31), "31 bits"), (dict(cols=2 ** 20 + 1), "20"), (dict(ty=3), "element type"), (dict(ty=-1), "element type"),
                          (dict(idb=2), "int32 or int64"), (dict(table=None), "null pointer"), (dict(ids=None), "null pointer"),
                          (dict(out=None), "null pointer"), (dict(ld=2), "overlap"), (dict(table=FAKE + 2), "alignment"),
                          (dict(ids=FAKE + 4), "alignment")):
@@ -428,13 +444,14 @@ def test_backward_arguments():
     L = _lib.lib()
     size = L.vings_row_lookup_backward_workspace_bytes
 
-    def call(n=4, rows=5000, cols=3, grad=FAKE, ld=3, ty=0, ids=FAKE, idb=8, out=FAKE, ot=0, ws=FAKE, ws_bytes=1 << 20):
+    def call(n=4, rows=5000, cols=3, grad=FAKE, ld=3, ty=0, ids=FAKE, idb=8, out=FAKE * 2, ot=0, ws=FAKE, ws_bytes=1 << 20):
         return L.vings_row_lookup_backward(n, rows, cols, grad, ld, ty, ids, idb, -1, 1.0, out, ot, None, 0, ws, ws_bytes, None)
     assert call(rows=0, out=None) == 0
     for change, text in ((dict(n=-1), "sizes"), (dict(cols=0), "sizes"), (dict(ot=1), "gradient's type"), (dict(ty=1, ot=2), "gradient's type"),
                          (dict(out=None), "null pointer"), (dict(grad=None), "null pointer"), (dict(ids=None), "null pointer"),
-                         (dict(ws=None), "null pointer"), (dict(ld=-1), "2^22"), (dict(ld=2 ** 22), "2^22"), (dict(ws=FAKE + 8), "256-byte"),
-                         (dict(ws_bytes=16), "too small"), (dict(out=FAKE + 2), "alignment"), (dict(grad=FAKE + 1), "alignment")):
+                         (dict(ws=None), "null pointer"), (dict(ld=-1), "2^20"), (dict(ld=2 ** 20 + 1), "2^20"),
+                         (dict(grad=FAKE * 2 - 4), "overlaps"), (dict(ids=FAKE * 2), "overlaps"), (dict(cols=2 ** 20 + 1), "20"), (dict(ws=FAKE + 8), "256-byte"),
+                         (dict(ws_bytes=16), "too small"), (dict(out=FAKE * 2 + 2), "alignment"), (dict(grad=FAKE + 1), "alignment")):
         assert call(**change) != 0 and text in _error(), change
     assert size(0, 9, 4, 0) == 0 and size(10, 9, 4, 9) == 0 and size(10, 0, 4, 0) == 0
     assert size(10, 5000, 4, 0) >= 80 and size(100000, 5000, 4, 0) >= 4 * 4 * 100000   # both sides of the passes

@@ -168,7 +168,7 @@ def ptr(t):
 
 
 def stream_ptr(device=None):
-    if device is not None and device.index is not None:
+    if isinstance(device, torch.device) and device.index is not None:
         return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 

@@ -25,8 +25,8 @@
 // workgroup sorts 1024 ids in LDS, sums their runs as in 2 and 3 and leaves one partial row per
 // row it met; a second launch adds those over the workgroups.  The gradient is then read in
 // stretches of 1024 rows instead of all over, and two launches replace seven (one, up to 1024 ids).
-// Sums are float32 over at most 64 terms in a row, then trees; the result is scaled and rounded
-// to the gradient's type once.
+// Sums are float32: at most 64 terms in a row in a lane group, then the scan, then the partial rows
+// of a run dealt out over the lane groups of its join; the result is scaled and rounded once.
 //
 // Serves per-keyframe rows that every splat reads through the keyframe that owns it
 // (globalkf_id, /root/reference/scripts/gaussian/gaussian_model.py:163-168) and any wide table;
@@ -47,6 +47,8 @@ constexpr int kTileItems = kTileIds / kTileThreads;
 constexpr int kFewRows = 4095;            // ... 12-bit keys, the one of ids without a row included
 constexpr int kFewTiles = 4096;           // ... partial rows that its join adds, at most
 constexpr int kPieceMax = 2048;           // sorted positions per workgroup of the segment kernel
+constexpr int64_t kMaxStride = 1 << 20;   // elements between gradient rows: byte offsets inside a
+static_assert(kMaxStride * 4 * (kTileIds - 1) < ((int64_t)1 << 32), "32-bit offsets");   // tile fit
 
 // ---------------------------------------------------------------------------
 // lookup
@@ -966,8 +968,8 @@ int lookup_by_id(int id_bytes, int64_t N, int64_t D, const void* table, int64_t 
 
 int check_shape(int64_t N, int64_t V, int64_t D, int type, int id_bytes) {
     VINGS_REQUIRE(N >= 0 && V >= 0 && D > 0, "sizes");
-    VINGS_REQUIRE(N < ((int64_t)1 << 31) && V < ((int64_t)1 << 31) - 1 && D < ((int64_t)1 << 22),
-                  "ids and rows must fit 31 bits, columns 22");
+    VINGS_REQUIRE(N < ((int64_t)1 << 31) && V < ((int64_t)1 << 31) - 1 && D <= kMaxStride,
+                  "ids and rows must fit 31 bits, columns 20");
     VINGS_REQUIRE(elem_known(type), "element type");
     VINGS_REQUIRE(id_bytes == 4 || id_bytes == 8, "ids are int32 or int64");
     return VINGS_OK;
@@ -985,7 +987,6 @@ extern "C" int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, c
     if (rc != VINGS_OK) return rc;
     if (n_ids == 0) return VINGS_OK;
     VINGS_REQUIRE((table || n_rows == 0) && ids && out, "null pointer");
-
     VINGS_REQUIRE(table_stride >= n_cols || n_rows <= 1, "rows must not overlap");
     VINGS_REQUIRE((((uintptr_t)table | (uintptr_t)out) & (elem_bytes(type) - 1)) == 0 &&
                       ((uintptr_t)ids & (id_bytes - 1)) == 0, "element alignment");
@@ -1003,7 +1004,7 @@ extern "C" int vings_row_lookup(int64_t n_ids, int64_t n_rows, int64_t n_cols, c
 extern "C" size_t vings_row_lookup_backward_workspace_bytes(int64_t n_ids, int64_t n_rows, int64_t n_cols,
                                                             int type) {
     const int64_t top = (int64_t)1 << 31;
-    if (n_ids <= 0 || n_rows <= 0 || n_cols <= 0 || n_ids >= top || n_cols >= (1 << 22) || !elem_known(type)) return 0;
+    if (n_ids <= 0 || n_rows <= 0 || n_cols <= 0 || n_ids >= top || n_cols > kMaxStride || !elem_known(type)) return 0;
     return carve_grad(nullptr, plan_segments(n_ids, n_rows, n_cols, type), n_ids, n_rows, n_cols).bytes;
 }
 
@@ -1028,7 +1029,15 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
         return VINGS_OK;
     }
     VINGS_REQUIRE(grad && ids, "null pointer");
-    VINGS_REQUIRE(grad_stride >= 0 && grad_stride < (1 << 22), "gradient rows lie less than 2^22 elements apart");
+    VINGS_REQUIRE(grad_stride >= 0 && grad_stride <= kMaxStride, "gradient rows lie at most 2^20 elements apart");
+    const auto apart = [&](const void* p, int64_t bytes) {     // ... from what the call writes
+        const uintptr_t a = (uintptr_t)p, r = (uintptr_t)rows, t = (uintptr_t)touched;
+        return (a + bytes <= r || r + F.bytes <= a) && (!touched || a + bytes <= t || t + n_rows <= a);
+    };
+    VINGS_REQUIRE(apart(grad, ((n_ids - 1) * grad_stride + n_cols) * elem_bytes(type)) && apart(ids, n_ids * id_bytes) &&
+                      (!touched || (uintptr_t)touched + n_rows <= (uintptr_t)rows ||
+                       (uintptr_t)rows + F.bytes <= (uintptr_t)touched),
+                  "what is written overlaps another array of the call");
     VINGS_REQUIRE(((uintptr_t)grad & (elem_bytes(type) - 1)) == 0 && ((uintptr_t)ids & (id_bytes - 1)) == 0,
                   "element alignment");
     VINGS_REQUIRE(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");

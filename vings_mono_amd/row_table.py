@@ -21,7 +21,7 @@ def _rows_2d(t):
     n = t.numel() // D
     if t.is_contiguous():
         return t, n, D
-    if t.dim() == 2 and (t.stride(1) == 1 or D == 1) and (n <= 1 or D <= t.stride(0) < 1 << 22 or t.stride(0) == 0):
+    if t.dim() == 2 and (t.stride(1) == 1 or D == 1) and (n <= 1 or D <= t.stride(0) <= 1 << 20 or t.stride(0) == 0):
         return t, n, t.stride(0) if n > 1 else D
     t = t.contiguous()
     return t, n, D

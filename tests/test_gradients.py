@@ -7,6 +7,7 @@ coefficient's and its own product's: 3 u + h_t, and half of float16's smallest s
 normal range."""
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -36,6 +37,11 @@ LISTS = {
     "odd": [((7, 3), torch.float32), ((5,), torch.bfloat16), ((0, 4), torch.float32), ((1, 1), torch.float16)],
     "chunk edges": [((n,), t) for n in (2047, 2048, 2049, 4096) for t in HALF],
     "splats": [((12345, w), torch.float32) for w in (3, 3, 1, 2, 4)],
+    "one workgroup": [((30720,), torch.float32), ((2047,), torch.bfloat16)],      # 16 chunks: its most
+    "two workgroups": [((30720,), torch.float32), ((2049,), torch.bfloat16)],
+    "112 tensors": [((100 + i,), torch.float32) for i in range(112)],             # one clipping launch
+    "113 tensors": [((100 + i,), torch.float16) for i in range(113)],
+    "161 tensors": [((3000 + i,), torch.float32) for i in range(161)],            # two norm launches
     "many": [((17 + 13 * i,), (torch.bfloat16, torch.float32, torch.float16)[i % 3]) for i in range(389)],
     "long": [((3000001,), torch.bfloat16), ((1500007,), torch.float32)],
 }
@@ -90,6 +96,41 @@ def test_short_gradients_stay_bit_for_bit():
     out = [torch.full_like(t, 7.0) for t in ts]
     gradients.clip_by_global_norm(ts, float("inf"), out=out)
     assert all(torch.equal(a, b) for a, b in zip(before, out))
+
+
+@gpu
+def test_some_in_place_and_some_not():
+    ts = make("splats")
+    before = [t.clone() for t in ts]
+    out = [ts[0], torch.empty_like(ts[1]), ts[2], torch.empty_like(ts[3]), ts[4]]
+    gradients.clip_by_global_norm(ts, 1.0, out=out)
+    alone = [torch.empty_like(t) for t in ts]
+    gradients.clip_by_global_norm(before, 1.0, out=alone)
+    assert all(torch.equal(a, b) for a, b in zip(out, alone))
+    assert torch.equal(ts[1], before[1]) and torch.equal(ts[3], before[3])
+
+
+@gpu
+def test_two_threads_on_two_streams():
+    """No state is shared between calls: each thread gets the bits of a solitary call."""
+    lists = [make("splats"), make("many")]
+    want = [gradients.global_norm(ts) for ts in lists]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got[k].append(gradients.global_norm(lists[k]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(got[k]) == 50 and all(torch.equal(g, want[k]) for g in got[k])
 
 
 @gpu
@@ -403,6 +444,12 @@ def test_step_edges_and_refusals():
         opt.step(vis, 100, max_norm=-1.0)
     with pytest.raises(_lib.VingsError):
         opt.step(vis, 100, max_norm=float("nan"))
+    moment = opt.state[params[0]]["exp_avg"]
+    for wrong in (moment.double(), moment[:50], moment.cpu()):
+        opt.state[params[0]]["exp_avg"] = wrong
+        with pytest.raises(_lib.VingsError):
+            opt.step(vis, 100, max_norm=1.0)
+    opt.state[params[0]]["exp_avg"] = moment
     guard = torch.tensor([11], dtype=torch.int32, device=DEV)
     norm = opt.step(vis, 100, guard=(guard.data_ptr(), 10), max_norm=1.0)       # does not fit: dropped
     assert float(norm) > 0 and all(torch.equal(a, b) for a, b in zip(params, before))

@@ -8,7 +8,7 @@ join's tree.  Partial rows: a piece of the sorted form holds 16 ids or more and 
 groups share them, a tile of the few-rows form holds one id of the row or more and at least
 sixteen groups share them, so a group adds count / 16 + 1 at most: (82 + count / 16) u of the sum
 of magnitudes, then u for the scale and h_t; float16 adds half its smallest step."""
-import ctypes
+import threading
 
 import pytest
 import torch
@@ -335,6 +335,31 @@ def test_other_stream_and_replayed_graph(n):
         e2, _ = row_table.lookup_rows_backward(g, ids, rows, scale=2.0)
         assert torch.equal(got, e) and torch.equal(touched, et) and torch.equal(got2, e2)
         assert torch.equal(out, row_table.lookup_rows(table, ids, scale=3.0))
+
+
+@gpu
+def test_two_threads_on_two_streams():
+    """No state is shared between calls: each thread gets the bits of a solitary call."""
+    cases = [(rand((40000, 12), seed=1), make_ids(40000, 80, "power"), 80),
+             (rand((9000, 136), torch.bfloat16, seed=2), make_ids(9000, 5000, "power"), 5000)]
+    want = [row_table.lookup_rows_backward(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(40):
+                got[k].append(row_table.lookup_rows_backward(*cases[k]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(got[k]) == 40
+        assert all(torch.equal(a, want[k][0]) and torch.equal(b, want[k][1]) for a, b in got[k])
 
 
 @gpu

@@ -617,8 +617,11 @@ class SparseGaussianAdam(torch.optim.Adam):
             state = self._moments(p)
             quad = (p, g.contiguous(), state["exp_avg"], state["exp_avg_sq"])
             keep.append(quad)
-            if not all([t.is_contiguous() and t.numel() == size for t in quad]):
-                raise _lib.VingsError("parameters and moments must be dense and of one size")
+            if not all([t.is_contiguous() and t.numel() == size and t.dtype is torch.float32
+                        and t.get_device() == index for t in quad]):
+                raise _lib.VingsError("parameters and moments must be dense float32 arrays of one size on one device")
+            if size // N > 0x7FFFFFFF:
+                raise _lib.VingsError("a row must hold fewer than 2^31 elements")
             arrays += [t.data_ptr() for t in quad]
             b1, b2 = group.get("betas", (0.9, 0.999))
             consts.append((size // N, group["lr"], b1, b2, group["eps"]))

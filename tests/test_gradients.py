@@ -484,6 +484,39 @@ def test_step_on_more_than_2_to_the_31_elements():
 
 
 @gpu
+@pytest.mark.parametrize("n,w", [((1 << 31) - 8000, 1), ((1 << 31) - 1, 1), ((1 << 30) + 1, 2), (715827890, 3)])
+def test_step_of_narrow_rows_by_64_bit_indexes(n, w):
+    """Four consecutive elements lie in up to four rows; every row keeps its own visibility."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("60 GB of free memory")
+    p, g, m, v = (torch.zeros((n, w), device=DEV) for _ in range(4))
+    vis = torch.zeros(n, dtype=torch.bool, device=DEV)
+    ends = [(0, (0, 2, 3, 5, 7)), (n - 9, (0, 1, 3, 6, 8))]
+    for first, rows in ends:
+        g[first:first + 9] = 1.0
+        for r in rows:
+            vis[first + r] = True
+    par = torch.nn.Parameter(p)
+    opt = surfel.SparseGaussianAdam([{"params": [par], "lr": 0.1}], lr=0.0, eps=1e-15)
+    opt.state[par] = {"step": torch.tensor(0.0), "exp_avg": m, "exp_avg_sq": v}
+    par.grad = g
+    norm = opt.step(vis, n, max_norm=1e9)
+    assert float(norm) == pytest.approx((10 * w) ** 0.5, rel=2 * U)
+    for first, rows in ends:
+        for t in (par.detach(), m, v):
+            moved = (t[first:first + 9] != 0).cpu()
+            assert torch.equal(moved, torch.tensor([r in rows for r in range(9)])[:, None].expand(9, w))
+    assert int((m[9:n - 9] != 0).sum()) == 0
+
+
+@gpu
+def test_step_of_more_rows_than_31_bits_is_refused():
+    opt, _ = optimizer(*adam_state(100, (3, 1), seed=6)[:4])
+    with pytest.raises(_lib.VingsError):
+        opt.step(torch.zeros((1 << 31) + 4, dtype=torch.bool, device=DEV), (1 << 31) + 4, max_norm=1.0)
+
+
+@gpu
 def test_captured_step():
     data = adam_state(20000, (3, 3, 1, 2, 4), seed=8)
     vis = data[4]

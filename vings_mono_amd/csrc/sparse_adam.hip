@@ -117,7 +117,7 @@ constexpr int kStepQuads = 2;          // flight together
 typedef Elem<float>::vec quad_t;       // 16-byte access at any 4-byte boundary
 
 // Which of the four elements from e0 (a multiple of 4, e0 + 4 <= N * width) lie in visible rows of
-// W floats (W = 0: of `width` floats).  Four elements touch four rows of one float, else two at
+// W floats (W = 0: of `width` >= 2 floats).  Four elements touch four rows of one float, else two at
 // most; the loads are not guarded (see below), the second row is clamped instead.
 template <int W, typename I>
 __device__ __forceinline__ int visible_quad(const uint8_t* __restrict__ visible, I e0, int N, int width) {
@@ -153,7 +153,8 @@ __device__ __forceinline__ void for_blocks(const AdamGroups& G, int N, int per_l
         const int64_t first = (b - G.first_block[g]) * 256 * per_lane;
         if (first < quads) {
             if (total > 0x7FFFFFFFll - 8192) {
-                f.template block<0, int64_t>(g, first, quads);
+                if (G.width[g] == 1) f.template block<1, int64_t>(g, first, quads);
+                else f.template block<0, int64_t>(g, first, quads);
             } else {
                 const uint32_t f32 = (uint32_t)first, q32 = (uint32_t)quads;
                 switch (G.width[g]) {

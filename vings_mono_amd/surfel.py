@@ -595,6 +595,8 @@ class SparseGaussianAdam(torch.optim.Adam):
     def _clipped_step(self, L, vis, N, guard, max_norm):
         if not max_norm >= 0.0:
             raise _lib.VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
+        if N > 0x7FFFFFFF:
+            raise _lib.VingsError(f"the step takes fewer than 2^31 rows (got {N})")
         dev, index = vis.device, vis.get_device()
         arrays, keep, consts = [], [], []
         for group in self.param_groups:

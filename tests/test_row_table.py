@@ -338,6 +338,27 @@ def test_other_stream_and_replayed_graph(n):
 
 
 @gpu
+def test_out_counts_as_written():
+    """A tensor that autograd saved and the call then overwrote is noticed in the backward pass."""
+    ids, g = make_ids(50, 7, "uniform"), rand((50, 3))
+    out = torch.ones((7, 3), device=DEV)
+    leaf = torch.ones((7, 3), device=DEV, requires_grad=True)
+    product = leaf * out
+    row_table.lookup_rows_backward(g, ids, 7, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("padding", [-1, -5, 7, 2 ** 63, 2 ** 64 + 3])
+def test_padding_id_that_names_no_row(padding):
+    ids, g = make_ids(500, 7, "strays"), rand((500, 3))
+    want, wt = row_table.lookup_rows_backward(g, ids, 7)
+    got, touched = row_table.lookup_rows_backward(g, ids, 7, padding_id=padding)
+    assert torch.equal(got, want) and torch.equal(touched, wt)
+
+
+@gpu
 def test_two_threads_on_two_streams():
     """No state is shared between calls: each thread gets the bits of a solitary call."""
     cases = [(rand((40000, 12), seed=1), make_ids(40000, 80, "power"), 80),

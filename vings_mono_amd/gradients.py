@@ -115,7 +115,7 @@ def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
     each of its input's type or float32 (clipped float32 gradients of a bfloat16 backward pass),
     overlapping nothing else of the call.  In place a gradient that is short enough is left
     unwritten.  NaN gradients give a NaN norm and NaN results; an infinite norm gives zeros (and
-    NaN where the gradient itself is infinite)."""
+    NaN where the gradient itself is infinite), or NaN if max_norm is infinite too."""
     kind = _kind(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -67,12 +67,14 @@ def _lookup_backward(grad, ids, num_rows, scale, padding_id, out, touched, keep_
     D = grad.shape[-1]
     src, n, ld = _rows_2d(grad)
     flat = ids.contiguous()
+    if padding_id is None or not 0 <= padding_id < num_rows:
+        padding_id = -1                  # names no row, like no padding id at all
     L, dev, et = _lib.lib(), grad.device, _lib.ELEM_TYPES[grad.dtype]
     with _lib.on_device(dev):
         ws = torch.empty(L.vings_row_lookup_backward_workspace_bytes(n, num_rows, D, et), dtype=torch.uint8, device=dev)
         check(L.vings_row_lookup_backward(
             n, num_rows, D, src.data_ptr(), ld, et, flat.data_ptr(), flat.element_size(),
-            -1 if padding_id is None else int(padding_id), scale, out.data_ptr(),
+            int(padding_id), scale, out.data_ptr(),
             _lib.ELEM_TYPES[out.dtype], None if touched is None else touched.data_ptr(),
             1 if keep_touched else 0, ws.data_ptr(), ws.numel(), stream_ptr(dev)),
             "vings_row_lookup_backward")
@@ -135,11 +137,14 @@ def lookup_rows_backward(grad, ids, num_rows, scale=1.0, padding_id=None, out=No
         raise VingsError(f"grad must have the shape of ids and one more dimension "
                          f"(got {tuple(grad.shape)} for ids {tuple(ids.shape)})")
     shape = (num_rows, grad.shape[-1])
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(shape, dtype=grad.dtype, device=grad.device)
     elif tuple(out.shape) != shape or not out.is_contiguous() or out.device != grad.device \
             or out.dtype not in (grad.dtype, torch.float32):
         raise VingsError(f"out must be a contiguous {shape} tensor of {grad.dtype} or float32 on {grad.device}")
     touched = torch.empty(num_rows, dtype=torch.bool, device=grad.device)
     _lookup_backward(grad, ids, num_rows, float(scale), padding_id, out, touched, False)
+    if given:
+        torch.autograd.graph.increment_version(out)
     return out, touched

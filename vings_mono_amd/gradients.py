@@ -39,7 +39,7 @@ def _dense(t):
     return True
 
 
-class _List:
+class TensorList:
     """A checked list of tensors and the tables the C entry points take."""
     __slots__ = ("tensors", "device", "contiguous", "n", "numels", "pointers", "types")
 
@@ -48,7 +48,12 @@ class _List:
         if not tensors:
             raise VingsError(f"{what}: no tensors given")
         self.device = tensors[0].device
-        types = list(map(_lib.ELEM_TYPES.get, map(_dtype, tensors)))
+        types = list(map(_dtype, tensors))
+        kinds = set(types)
+        if len(kinds) == 1:
+            types = [_lib.ELEM_TYPES.get(types[0])] * len(types)
+        else:
+            types = list(map(_lib.ELEM_TYPES.get, types))
         if None in types or set(map(_get_device, tensors)) != {self.device.index}:
             self._refuse(what)
         try:
@@ -99,7 +104,7 @@ def global_norm(tensors, norm_type=2.0):
     norm_type=inf.  Sums are held in 64 bits: no overflow below the largest float32 norm.  A
     tensor given twice counts twice."""
     kind = _kind(norm_type)
-    g = _List(tensors, "global_norm")
+    g = TensorList(tensors, "global_norm")
     L, numels = _lib.lib(), _address(g.numels)
     with _lib.on_device(g.device):
         nbytes = L.vings_grad_norm_workspace_bytes(g.n, numels)
@@ -120,10 +125,10 @@ def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
-    g = _List(tensors, "clip_by_global_norm")
+    g = TensorList(tensors, "clip_by_global_norm")
     o = g
     if out is not None:
-        o = _List(out, "clip_by_global_norm: out")
+        o = TensorList(out, "clip_by_global_norm: out")
         if o.n != g.n or o.device != g.device:
             raise VingsError("out must hold one tensor per gradient, on the gradients' device")
         for t, u in zip(g.tensors, o.tensors):

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import check, ptr, stream_ptr
-from .gradients import norm_and_workspace
+from .gradients import TensorList, norm_and_workspace
 
 GEOM_STRIDE = 24
 GRAD_STRIDE = 20
@@ -597,8 +597,8 @@ class SparseGaussianAdam(torch.optim.Adam):
             raise _lib.VingsError(f"max_norm must not be negative or NaN (got {max_norm})")
         if N > 0x7FFFFFFF:
             raise _lib.VingsError(f"the step takes fewer than 2^31 rows (got {N})")
-        dev, index = vis.device, vis.get_device()
-        arrays, keep, consts = [], [], []
+        dev = vis.device
+        params, grads, ms, vs, widths, consts = [], [], [], [], [], []
         for group in self.param_groups:
             if len(group["params"]) != 1:
                 raise _lib.VingsError("more than one tensor in group")
@@ -606,39 +606,38 @@ class SparseGaussianAdam(torch.optim.Adam):
             g = p.grad
             if g is None:
                 continue
-            _lib.require_gpu_tensor(p, "param", torch.float32)
-            if p.get_device() != index or g.get_device() != index:
-                raise _lib.VingsError("parameters, gradients and visibility must live on one device")
-            if g.dtype != torch.float32:
-                raise _lib.VingsError(f"gradients must be float32 (got {g.dtype})")
             size = p.numel()
             if N == 0 or size == 0:
                 continue
-            if size % N != 0:
-                raise _lib.VingsError("parameter size is not a multiple of N")
+            width, rest = divmod(size, N)
+            if rest or width > 0x7FFFFFFF:
+                raise _lib.VingsError("parameter size is not a multiple of N, or 2^31 times N and more")
             state = self._moments(p)
-            quad = (p, g.contiguous(), state["exp_avg"], state["exp_avg_sq"])
-            keep.append(quad)
-            if not all([t.is_contiguous() and t.numel() == size and t.dtype is torch.float32
-                        and t.get_device() == index for t in quad]):
-                raise _lib.VingsError("parameters and moments must be dense float32 arrays of one size on one device")
-            if size // N > 0x7FFFFFFF:
-                raise _lib.VingsError("a row must hold fewer than 2^31 elements")
-            arrays += [t.data_ptr() for t in quad]
+            params.append(p)
+            grads.append(g.contiguous())
+            ms.append(state["exp_avg"])
+            vs.append(state["exp_avg_sq"])
+            widths.append(width)
             b1, b2 = group.get("betas", (0.9, 0.999))
-            consts.append((size // N, group["lr"], b1, b2, group["eps"]))
-        n = len(consts)
+            consts.append((group["lr"], b1, b2, group["eps"]))
+        n = len(widths)
         if n == 0:
             return torch.zeros((), dtype=torch.float32, device=dev)
-        widths, lrs, b1s, b2s, epss = zip(*consts)
-        tables = [array.array("Q", arrays[k::4]) for k in range(4)]
-        tables += [array.array("i", widths), array.array("f", lrs), array.array("d", b1s), array.array("d", b2s),
-                   array.array("f", epss)]
+        arrays = TensorList(params + grads + ms + vs, "clipped step")
+        if arrays.device != dev:
+            raise _lib.VingsError(f"parameters and visibility must live on one device ({arrays.device} and {dev})")
+        if any(arrays.types) or not arrays.contiguous or arrays.numels != arrays.numels[:n] * 4:
+            raise _lib.VingsError("parameters, gradients and moments must be dense float32 arrays of one size")
+        base = arrays.pointers.buffer_info()[0]
+        lrs, b1s, b2s, epss = zip(*consts)
+        tables = [array.array("i", widths), array.array("f", lrs), array.array("d", b1s), array.array("d", b2s),
+                  array.array("f", epss)]
         with _lib.on_device(dev):
             nbytes = L.vings_sparse_adam_clipped_workspace_bytes(n)
             norm, ws = norm_and_workspace(nbytes, dev)
             check(L.vings_sparse_adam_clipped(
-                n, *[t.buffer_info()[0] for t in tables], ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
+                n, base, base + 8 * n, base + 16 * n, base + 24 * n, *[t.buffer_info()[0] for t in tables],
+                ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
                 None if guard is None else guard[0], 0 if guard is None else int(guard[1]),
                 stream_ptr(dev)), "vings_sparse_adam_clipped")
         return norm

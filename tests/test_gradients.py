@@ -37,8 +37,8 @@ LISTS = {
     "odd": [((7, 3), torch.float32), ((5,), torch.bfloat16), ((0, 4), torch.float32), ((1, 1), torch.float16)],
     "chunk edges": [((n,), t) for n in (2047, 2048, 2049, 4096) for t in HALF],
     "splats": [((12345, w), torch.float32) for w in (3, 3, 1, 2, 4)],
-    "one workgroup": [((30720,), torch.float32), ((2047,), torch.bfloat16)],      # 16 chunks: its most
-    "two workgroups": [((30720,), torch.float32), ((2049,), torch.bfloat16)],
+    "one workgroup": [((30719,), torch.float32), ((2047,), torch.bfloat16)],      # 16 chunks: its most
+    "two workgroups": [((30719,), torch.float32), ((2049,), torch.bfloat16)],
     "112 tensors": [((100 + i,), torch.float32) for i in range(112)],             # one clipping launch
     "113 tensors": [((100 + i,), torch.float16) for i in range(113)],
     "161 tensors": [((3000 + i,), torch.float32) for i in range(161)],            # two norm launches

@@ -12,7 +12,8 @@
 //      behind the last row.  Up to 32768 ids workgroups sort runs of 1024 in LDS and a second
 //      launch merges the runs, every id finding its place by bisection in each of them, while
 //      further workgroups of both launches clear dtable and touched; more ids take the tile
-//      passes of radix_sort.hpp, 8 bits each
+//      passes of radix_sort.hpp, 8 bits each (clearing beside the first; 100 k ids into 60 k rows
+//      of 16 float32: 42 us with clearing and every scan in launches of their own, now 36)
 //   2. segment kernel: the sorted positions are cut into pieces of equal length, whatever rows
 //      they belong to, so one frequent id costs no more than many rare ones.  A lane group walks
 //      a few consecutive positions, holds its columns' sum in float32 registers, and writes a
@@ -180,6 +181,18 @@ __device__ __forceinline__ void clear(const Fill& F, int64_t t, int64_t n) {
 
 __global__ __launch_bounds__(256) void row_clear_kernel(Fill F) {
     clear(F, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
+// The first pass's histograms in workgroups [0, ntiles), the others clear.
+template <typename I, bool DIRECT>
+__global__ __launch_bounds__(kSortThreads) void row_first_hist_kernel(const I* __restrict__ ids, int64_t N, int ntiles,
+                                                                      uint32_t* __restrict__ thist, IdRange range,
+                                                                      Fill F) {
+    if ((int)blockIdx.x >= ntiles)
+        clear(F, (int64_t)(blockIdx.x - ntiles) * kSortThreads + threadIdx.x,
+              (int64_t)(gridDim.x - ntiles) * kSortThreads);
+    else
+        sort_tile_hist<I, DIRECT>(ids, N, 0, ntiles, thist, range);
 }
 
 // Stable counting sort of one digit inside a workgroup: the place of this lane's ITEMS keys
@@ -864,33 +877,44 @@ int sort_runs(const I* ids, int N, IdRange range, int bits, const GradWorkspace&
 }
 
 // Leaves the sorted pairs in key[*at], val[*at].
-template <typename I>
-int sort_tiles(const I* ids, int64_t N, IdRange range, int bits, const GradWorkspace& w, int* at,
+template <typename I, bool DIRECT>
+int sort_tiles(const I* ids, int64_t N, IdRange range, int bits, const GradWorkspace& w, const Fill& F, int* at,
                hipStream_t s) {
     const int ntiles = cdiv(N, kSortTile);
     int cur = 1;
     for (int shift = 0; shift < bits; shift += kRadixBits) {
         const int nbits = std::min(kRadixBits, bits - shift);
         if (shift == 0)
-            sort_tile_hist_kernel<I><<<ntiles, kSortThreads, 0, s>>>(ids, N, 0, ntiles, w.thist, nullptr, range);
+            row_first_hist_kernel<I, DIRECT><<<ntiles + clear_grid(F), kSortThreads, 0, s>>>(ids, N, ntiles, w.thist,
+                                                                                             range, F);
         else
-            sort_tile_hist_kernel<uint32_t><<<ntiles, kSortThreads, 0, s>>>(w.key[cur], N, shift, ntiles, w.thist,
-                                                                            nullptr, range);
+            sort_tile_hist_kernel<uint32_t, DIRECT><<<ntiles, kSortThreads, 0, s>>>(w.key[cur], N, shift, ntiles,
+                                                                                    w.thist, nullptr, range);
         VINGS_LAUNCH_CHECK();
-        sort_scan_kernel<<<kRadix, 256, 0, s>>>(w.thist, ntiles, w.totals);
-        VINGS_LAUNCH_CHECK();
+        if (!DIRECT) {
+            sort_scan_kernel<<<kRadix, 256, 0, s>>>(w.thist, ntiles, w.totals);
+            VINGS_LAUNCH_CHECK();
+        }
         if (shift == 0)
-            sort_scatter_kernel<I><<<ntiles, kSortThreads, 0, s>>>(ids, nullptr, w.key[cur ^ 1], w.val[cur ^ 1], N, 0,
-                                                                   ntiles, w.thist, w.totals, nullptr, nbits, range);
+            sort_scatter_kernel<I, DIRECT><<<ntiles, kSortThreads, 0, s>>>(
+                ids, nullptr, w.key[cur ^ 1], w.val[cur ^ 1], N, 0, ntiles, w.thist, w.totals, nullptr, nbits, range);
         else
-            sort_scatter_kernel<uint32_t><<<ntiles, kSortThreads, 0, s>>>(w.key[cur], w.val[cur], w.key[cur ^ 1],
-                                                                          w.val[cur ^ 1], N, shift, ntiles, w.thist,
-                                                                          w.totals, nullptr, nbits, range);
+            sort_scatter_kernel<uint32_t, DIRECT><<<ntiles, kSortThreads, 0, s>>>(
+                w.key[cur], w.val[cur], w.key[cur ^ 1], w.val[cur ^ 1], N, shift, ntiles, w.thist, w.totals, nullptr,
+                nbits, range);
         VINGS_LAUNCH_CHECK();
         cur ^= 1;
     }
     *at = cur;
     return VINGS_OK;
+}
+
+template <typename I>
+int sort_ids(const I* ids, int64_t N, IdRange range, int bits, const GradWorkspace& w, const Fill& F, int* at,
+             hipStream_t s) {
+    if (N <= kMergeSortMax) return sort_runs<I>(ids, (int)N, range, bits, w, F, at, s);
+    return N <= (int64_t)kDirectTiles * kSortTile ? sort_tiles<I, true>(ids, N, range, bits, w, F, at, s)
+                                                  : sort_tiles<I, false>(ids, N, range, bits, w, F, at, s);
 }
 
 template <typename T, typename O, int V>
@@ -1067,16 +1091,9 @@ extern "C" int vings_row_lookup_backward(int64_t n_ids, int64_t n_rows, int64_t 
             ? few_by_kind<_Float16, float>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s)
             : few_by_kind<_Float16, _Float16>(S, p, w, grad, ids, id_bytes, range, bits, rows, keep_touched, s);
     }
-    int at = 0, rs;
-    if (n_ids <= kMergeSortMax) {
-        rs = id_bytes == 8 ? sort_runs((const int64_t*)ids, (int)n_ids, range, bits, w, F, &at, s)
-                           : sort_runs((const int32_t*)ids, (int)n_ids, range, bits, w, F, &at, s);
-    } else {
-        row_clear_kernel<<<clear_grid(F), 256, 0, s>>>(F);
-        VINGS_LAUNCH_CHECK();
-        rs = id_bytes == 8 ? sort_tiles((const int64_t*)ids, n_ids, range, bits, w, &at, s)
-                           : sort_tiles((const int32_t*)ids, n_ids, range, bits, w, &at, s);
-    }
+    int at = 0;
+    const int rs = id_bytes == 8 ? sort_ids((const int64_t*)ids, n_ids, range, bits, w, F, &at, s)
+                                 : sort_ids((const int32_t*)ids, n_ids, range, bits, w, F, &at, s);
     if (rs != VINGS_OK) return rs;
     VINGS_REQUIRE((256 >> p.lg) * p.per_group <= kPieceMax, "piece");
     S.keys = w.key[at];

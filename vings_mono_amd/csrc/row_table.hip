@@ -789,19 +789,26 @@ SegmentPlan plan_segments(int64_t N, int64_t rows, int64_t D, int type) {
     p.lg = vectors >= 64 ? 6 : ceil_log2(vectors);
     p.segments = (int)((vectors + (1 << p.lg) - 1) >> p.lg);
     // few rows: a lane group of the tile sums at most 64 positions, the tiles' tables of the rows
-    // they met stay below 16 MB, and the partial rows (as many as a tile has ids, at most) cost less
-    // than the sorted form's passes, about 45 us, in which HBM moves 256 MB.  Measured at 1 M ids
-    // of 64 float32 columns: 300 rows 90 us, 1000 rows 118 us; sorted 99 us whatever the rows
+    // they met stay below 16 MB, and what the two launches move for their split costs less than
+    // the sorted form's passes.  They write and read the partial rows (as many as a tile has ids,
+    // at most), and the join of more than 256 rows picks two bytes out of a line for every tile
+    // and row; a pass costs what moving 64 MB and 90 bytes an id does.  Measured at 1 M ids, few
+    // against sorted: 1000 rows of 12 float32 46 and 69 us, of 32 60 and 69; 2000 rows of 32 72
+    // and 70, 4000 rows 90 and 69; 200 rows of 64 78 and 77, 500 rows 97 and 94, 2000 153 and 96.
+    // At 250 k ids 4000 rows of 64 take 46 and 49 us
     const int64_t tiles = (N + kTileIds - 1) / kTileIds;
+    p.by_row = rows <= 256;
+    const int64_t passes = rows < kRadix ? 1 : 2;
+    const int64_t split = 2 * tiles * std::min<int64_t>(rows, kTileIds) * D * 4 + (p.by_row ? 0 : 64 * tiles * rows);
     p.few = rows <= kFewRows && vectors <= 16 && tiles <= kFewTiles && tiles * rows <= (1 << 23) &&
-            2 * tiles * std::min<int64_t>(rows, kTileIds) * D * 4 <= ((int64_t)1 << 28);
+            split <= passes * ((64 << 20) + 90 * N);
     if (p.few) {
         const int groups = kTileThreads >> p.lg;
         p.per_group = (int)((std::min<int64_t>(N, kTileIds) + groups - 1) / groups);
         p.pieces = (int)tiles;
-        p.by_row = rows <= 256;
         return p;
     }
+    p.by_row = false;
     const int groups = 256 >> p.lg;
     // about 2048 workgroups (eight per CU) where there are enough ids; 4 positions at least (the
     // loads a lane keeps in flight), 64 at most (what one float32 sum may run over)

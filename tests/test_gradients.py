@@ -39,6 +39,8 @@ LISTS = {
     "splats": [((12345, w), torch.float32) for w in (3, 3, 1, 2, 4)],
     "one workgroup": [((30719,), torch.float32), ((2047,), torch.bfloat16)],      # 16 chunks: its most
     "two workgroups": [((30719,), torch.float32), ((2049,), torch.bfloat16)],
+    "16 tensors": [((5000 + i,), torch.bfloat16) for i in range(16)],             # the short table
+    "17 tensors": [((5000 + i,), torch.bfloat16) for i in range(17)],
     "112 tensors": [((100 + i,), torch.float32) for i in range(112)],             # one clipping launch
     "113 tensors": [((100 + i,), torch.float16) for i in range(113)],
     "161 tensors": [((3000 + i,), torch.float32) for i in range(161)],            # two norm launches

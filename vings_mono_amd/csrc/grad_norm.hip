@@ -31,6 +31,8 @@ namespace vings {
 constexpr int kChunk = 2048;              // elements
 constexpr int kNormTensors = 160;         // per launch: 3.4 KB of kernel arguments
 constexpr int kClipTensors = 112;         // ... 3.4 KB
+constexpr int kFewTensors = 16;           // a list this short travels in 0.5 KB and starts sooner
+                                          // (norm of 5 tensors 10.6 -> 10.3 us, clipping 19.7 -> 19.4)
 constexpr int kMaxPartials = 1024;        // workgroups per launch
 constexpr int kOneBlockChunks = 16;
 
@@ -166,7 +168,8 @@ __device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t o
 
 // A gradient that is already short enough stays as it is: in place, nothing is read or written.
 // The chunks are taken from the last to the first: what the norm read last is still in the cache.
-__device__ __forceinline__ void range_scale(const TensorTable<kClipTensors, true>& T, uint32_t lo,
+template <int CAP>
+__device__ __forceinline__ void range_scale(const TensorTable<CAP, true>& T, uint32_t lo,
                                             uint32_t hi, int waves, float coef) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (hi <= lo + w) return;
@@ -218,13 +221,13 @@ __global__ __launch_bounds__(1024) void norm_final_kernel(const double* __restri
     if (threadIdx.x == 0) *norm = v;
 }
 
-template <int KIND>
-__global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<kClipTensors, true> args,
+template <int KIND, int CAP>
+__global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<CAP, true> args,
                                                          const double* __restrict__ partial,
                                                          int n_partial, float max_norm,
                                                          float* __restrict__ norm) {
     __shared__ double scratch[16];
-    __shared__ TensorTable<kClipTensors, true> T;
+    __shared__ TensorTable<CAP, true> T;
     copy_table(args, T);
     const float v = norm_of_partials<KIND>(partial, n_partial, scratch);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
@@ -234,12 +237,12 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<kClipTensor
 }
 
 // Norm and scaling of a few chunks by one workgroup.
-template <int KIND>
-__global__ __launch_bounds__(1024) void clip_one_block_kernel(TensorTable<kClipTensors, true> args,
+template <int KIND, int CAP>
+__global__ __launch_bounds__(1024) void clip_one_block_kernel(TensorTable<CAP, true> args,
                                                               float max_norm,
                                                               float* __restrict__ norm) {
     __shared__ double scratch[16];
-    __shared__ TensorTable<kClipTensors, true> T;
+    __shared__ TensorTable<CAP, true> T;
     copy_table(args, T);
     const int waves = blockDim.x >> 6;
     const uint32_t hi = T.first[T.count];
@@ -360,10 +363,10 @@ int launch_partials(const ListPlan& p, const void* const* in, void* const* out, 
     return VINGS_OK;
 }
 
-template <int KIND>
+template <int KIND, int CAP>
 int norm_impl(int n_tensors, const void* const* in, const int64_t* n, const int* types, float* norm,
               void* workspace, hipStream_t s) {
-    const ListPlan p = plan_list(n_tensors, n, kNormTensors);
+    const ListPlan p = plan_list(n_tensors, n, CAP);
     ProfScope prof(PROF_AUX, s);
     if (p.chunks == 0) {
         norm_of_nothing_kernel<<<1, 1, 0, s>>>(norm);
@@ -371,24 +374,24 @@ int norm_impl(int n_tensors, const void* const* in, const int64_t* n, const int*
         return VINGS_OK;
     }
     if (p.launch_end.size() == 1 && p.chunks <= kOneBlockChunks) {
-        TensorTable<kNormTensors, false> T;
+        TensorTable<CAP, false> T;
         fill_table(T, p, 0, in, nullptr, n, types, nullptr);
-        norm_partial_kernel<KIND, kNormTensors, false><<<1, 64 * (int)p.chunks, 0, s>>>(T, nullptr, norm);
+        norm_partial_kernel<KIND, CAP, false><<<1, 64 * (int)p.chunks, 0, s>>>(T, nullptr, norm);
         VINGS_LAUNCH_CHECK();
         return VINGS_OK;
     }
     double* partials = (double*)workspace;
-    const int rc = launch_partials<KIND, kNormTensors, false>(p, in, nullptr, n, types, nullptr, partials, s);
+    const int rc = launch_partials<KIND, CAP, false>(p, in, nullptr, n, types, nullptr, partials, s);
     if (rc != VINGS_OK) return rc;
     norm_final_kernel<KIND><<<1, 1024, 0, s>>>(partials, (int)p.partials, norm);
     VINGS_LAUNCH_CHECK();
     return VINGS_OK;
 }
 
-template <int KIND>
+template <int KIND, int CAP>
 int clip_impl(int n_tensors, const void* const* in, void* const* out, const int64_t* n, const int* types,
               const int* out_types, float max_norm, float* norm, void* workspace, hipStream_t s) {
-    const ListPlan p = plan_list(n_tensors, n, kClipTensors);
+    const ListPlan p = plan_list(n_tensors, n, CAP);
     ProfScope prof(PROF_AUX, s);
     if (p.chunks == 0) {
         norm_of_nothing_kernel<<<1, 1, 0, s>>>(norm);
@@ -396,19 +399,19 @@ int clip_impl(int n_tensors, const void* const* in, void* const* out, const int6
         return VINGS_OK;
     }
     if (p.launch_end.size() == 1 && p.chunks <= kOneBlockChunks) {
-        TensorTable<kClipTensors, true> T;
+        TensorTable<CAP, true> T;
         fill_table(T, p, 0, in, out, n, types, out_types);
-        clip_one_block_kernel<KIND><<<1, 64 * (int)p.chunks, 0, s>>>(T, max_norm, norm);
+        clip_one_block_kernel<KIND, CAP><<<1, 64 * (int)p.chunks, 0, s>>>(T, max_norm, norm);
         VINGS_LAUNCH_CHECK();
         return VINGS_OK;
     }
     double* partials = (double*)workspace;
-    const int rc = launch_partials<KIND, kClipTensors, true>(p, in, out, n, types, out_types, partials, s);
+    const int rc = launch_partials<KIND, CAP, true>(p, in, out, n, types, out_types, partials, s);
     if (rc != VINGS_OK) return rc;
     for (int l = 0; l < (int)p.launch_end.size(); ++l) {
-        TensorTable<kClipTensors, true> T;
+        TensorTable<CAP, true> T;
         fill_table(T, p, l, in, out, n, types, out_types);
-        clip_scale_kernel<KIND><<<blocks_for(p.launch_chunks[l]), 256, 0, s>>>(
+        clip_scale_kernel<KIND, CAP><<<blocks_for(p.launch_chunks[l]), 256, 0, s>>>(
             T, partials, (int)p.partials, max_norm, l == 0 ? norm : nullptr);
         VINGS_LAUNCH_CHECK();
     }
@@ -448,9 +451,11 @@ extern "C" int vings_grad_norm(int n_tensors, const void* const* grads_host,
     VINGS_REQUIRE(((uintptr_t)workspace & 7) == 0, "workspace must be 8-byte aligned");
     VINGS_REQUIRE(workspace || workspace_bytes == 0, "null pointer");
     try {
-        return norm_kind == NORM_2
-            ? norm_impl<NORM_2>(n_tensors, grads_host, numels_host, types_host, norm, workspace, (hipStream_t)stream)
-            : norm_impl<NORM_MAX>(n_tensors, grads_host, numels_host, types_host, norm, workspace, (hipStream_t)stream);
+        const bool few = n_tensors <= kFewTensors;
+        const auto impl = norm_kind == NORM_2
+            ? (few ? norm_impl<NORM_2, kFewTensors> : norm_impl<NORM_2, kNormTensors>)
+            : (few ? norm_impl<NORM_MAX, kFewTensors> : norm_impl<NORM_MAX, kNormTensors>);
+        return impl(n_tensors, grads_host, numels_host, types_host, norm, workspace, (hipStream_t)stream);
     } catch (const std::exception& e) {
         set_error("gradient norm: %s", e.what());
         return VINGS_ERR_ARG;
@@ -484,11 +489,12 @@ extern "C" int vings_grad_clip(int n_tensors, const void* const* grads_host, voi
     try {
         VINGS_REQUIRE(!writes_overlap(n_tensors, grads_host, outs_host, numels_host, types_host, out_types_host),
                       "a clipped gradient overlaps another tensor of the call");
-        return norm_kind == NORM_2
-            ? clip_impl<NORM_2>(n_tensors, grads_host, outs_host, numels_host, types_host, out_types_host,
-                                max_norm, norm, workspace, (hipStream_t)stream)
-            : clip_impl<NORM_MAX>(n_tensors, grads_host, outs_host, numels_host, types_host, out_types_host,
-                                  max_norm, norm, workspace, (hipStream_t)stream);
+        const bool few = n_tensors <= kFewTensors;
+        const auto impl = norm_kind == NORM_2
+            ? (few ? clip_impl<NORM_2, kFewTensors> : clip_impl<NORM_2, kClipTensors>)
+            : (few ? clip_impl<NORM_MAX, kFewTensors> : clip_impl<NORM_MAX, kClipTensors>);
+        return impl(n_tensors, grads_host, outs_host, numels_host, types_host, out_types_host, max_norm, norm,
+                    workspace, (hipStream_t)stream);
     } catch (const std::exception& e) {
         set_error("gradient clip: %s", e.what());
         return VINGS_ERR_ARG;

@@ -71,12 +71,13 @@ def _lookup_backward(grad, ids, num_rows, scale, padding_id, out, touched, keep_
         padding_id = -1                  # names no row, like no padding id at all
     L, dev, et = _lib.lib(), grad.device, _lib.ELEM_TYPES[grad.dtype]
     with _lib.on_device(dev):
-        ws = torch.empty(L.vings_row_lookup_backward_workspace_bytes(n, num_rows, D, et), dtype=torch.uint8, device=dev)
+        nbytes = L.vings_row_lookup_backward_workspace_bytes(n, num_rows, D, et)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         check(L.vings_row_lookup_backward(
             n, num_rows, D, src.data_ptr(), ld, et, flat.data_ptr(), flat.element_size(),
             int(padding_id), scale, out.data_ptr(),
             _lib.ELEM_TYPES[out.dtype], None if touched is None else touched.data_ptr(),
-            1 if keep_touched else 0, ws.data_ptr(), ws.numel(), stream_ptr(dev)),
+            1 if keep_touched else 0, None if ws is None else ws.data_ptr(), nbytes, stream_ptr(dev)),
             "vings_row_lookup_backward")
 
 

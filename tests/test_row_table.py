@@ -122,6 +122,20 @@ def test_backward(n, rows, cols, how):
 
 
 @gpu
+@pytest.mark.parametrize("how", ["uniform", "one", "strays"])
+@pytest.mark.parametrize("n,rows,cols", [(n, r, c) for n in (131071, 131072, 131073, 300001)
+                                         for r, c in ((5000, 8), (70000, 5), (4000, 72))] + [(4300001, 70000, 5)])
+def test_sort_by_tiles(n, rows, cols, how):
+    """Up to 64 tiles of 2048 ids and above; 4 300 001 ids are two rounds of the scan."""
+    grad, ids = rand((n, cols), seed=cols), make_ids(n, rows, how)
+    out = torch.full((rows, cols), 9.0, device=DEV)
+    got, touched = row_table.lookup_rows_backward(grad, ids, rows, out=out)
+    check_backward(grad, ids, rows, 1.0, got, touched)
+    again, _ = row_table.lookup_rows_backward(grad, ids.int() if how == "uniform" else ids, rows)
+    assert torch.equal(again, got)
+
+
+@gpu
 @pytest.mark.parametrize("bits", [1, 7, 8, 9, 16, 17, 24, 30])
 @pytest.mark.parametrize("n", [700, 3000, 12000, 40000])
 def test_sort_over_every_number_of_passes(n, bits):

@@ -243,7 +243,8 @@ int vings_sparse_adam_multi(int n_groups, float* const* params_host,
  * that shares a 16-byte quad with a visible row is written back unchanged).  A norm
  * that is infinite or NaN skips the step on the device: parameters and moments stay.  The
  * factors 1-b1 and 1-b2 are formed in 64 bits (vings_sparse_adam* form them in float32).  `norm`
- * (device, one float) receives the norm before clipping in every case.  Up to 64 groups, each
+ * (device, one float) receives the norm before clipping, and infinity for a step that the guard
+ * drops: a step was skipped exactly if its norm is not finite.  Up to 64 groups, each
  * with its own b1, b2 and eps; arrays need 4-byte alignment only.  `instance_count` (may be
  * NULL) and `capacity`: as in vings_sparse_adam_multi_guarded.  The workspace holds the partial
  * sums of the norm; nothing in it outlives the call. */

@@ -585,6 +585,51 @@ def test_mapper_view_steps_clip():
         assert nf > 0 and abs(nf - ng) <= 1e-2 * nf
 
 
+@gpu
+def test_a_dropped_step_reports_no_norm():
+    """The gradients of a step that its guard drops are incomplete, or another step's: their norm is
+    none of this step's.  Infinity says so, as the norm of every skipped step is not finite."""
+    ps, gs, ms, vs, vis = adam_state(5000, (3, 1), seed=16)
+    opt, params = optimizer(ps, gs, ms, vs)
+    guard = torch.tensor([11], dtype=torch.int32, device=DEV)
+    first = float(opt.step(vis, 5000, guard=(guard.data_ptr(), 11), max_norm=1.0))
+    assert math.isfinite(first) and first > 0
+    before = [x.clone() for p in params for x in (p.detach(), *list(opt.state[p].values())[1:])]
+    assert float(opt.step(vis, 5000, guard=(guard.data_ptr(), 10), max_norm=1.0)) == math.inf
+    after = [x for p in params for x in (p.detach(), *list(opt.state[p].values())[1:])]
+    assert all(torch.equal(x, y) for x, y in zip(before, after))
+    gs[0][int(vis.nonzero()[0]), 0] = float("nan")               # ... whatever they hold
+    assert float(opt.step(vis, 5000, guard=(guard.data_ptr(), 10), max_norm=1.0)) == math.inf
+
+
+@gpu
+def test_a_dropped_view_step_reports_no_norm():
+    """The same of a captured view whose instances outgrew its graph, behind a step of another view."""
+    intr = synth.intrinsic_for(256, 160)
+    raw = synth.make_splats(5000, 256, 160, n_views=2, seed=72)
+    mapper = harness.SurfelMapper(raw, DEV, max_grad_norm=0.1)
+    views = []
+    for c2w in synth.window_poses(2):
+        w2c = torch.linalg.inv(c2w).to(DEV)
+        with torch.no_grad():
+            pr = harness.render({k: v.to(DEV) for k, v in synth.perturb_splats(raw).items()}, w2c, intr)
+        gt = {"rgb": pr["rgb"].clone(), "depth": pr["depth"].clone(), "depth_cov": torch.ones_like(pr["depth"])}
+        views.append((harness.view_settings(w2c, intr), gt, w2c[:3, :3].cpu()))
+    step = lambda k: mapper.fused_view_graphed(k, views[k][0], intr, views[k][1], views[k][2], k)
+    step(0), step(1)
+    ent = mapper._view_graphs[0]
+    assert ent["D"] > 8000
+    ent["D"] = 64
+    step(0)                                                      # captured with too little room: dropped
+    torch.cuda.synchronize()
+    assert int(ent["count"][2]) > ent["capacity"]
+    assert float(mapper.last_grad_norm) == math.inf
+    step(1)
+    assert 0 < float(mapper.last_grad_norm) < math.inf
+    step(0)                                                      # repeated, and captured with room
+    assert 0 < float(mapper.last_grad_norm) < math.inf
+
+
 def test_compact_exchange_refuses_clipping():
     class Reducer:
         world, compact, n = 2, True, 4

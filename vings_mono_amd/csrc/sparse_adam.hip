@@ -275,10 +275,11 @@ __global__ __launch_bounds__(256) void sparse_adam_clipped_kernel(
     const double* __restrict__ partial, int n_partial, float max_norm, float* __restrict__ norm_out,
     const uint32_t* __restrict__ guard_count, uint32_t guard_limit) {
     __shared__ double scratch[16];
-    const float norm = norm_of_partials<NORM_2>(partial, n_partial, scratch);
+    // (a dropped step's gradients are incomplete, or those of the step before: it has no norm)
+    const bool dropped = guard_count && *guard_count > guard_limit;
+    const float norm = dropped ? __builtin_inff() : norm_of_partials<NORM_2>(partial, n_partial, scratch);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     if (!(norm <= 3.402823466e+38f)) return;                    // infinite or NaN: no step
-    if (guard_count && *guard_count > guard_limit) return;
     for_blocks(G, N, kStepQuads, ClippedUpdate{G, visible, N, C, clip_coefficient(norm, max_norm)});
 }
 

@@ -244,7 +244,8 @@ class SurfelMapper:
                  max_grad_norm=None):
         """`max_grad_norm`: every view step clips its gradients by their global norm over the
         splats it steps (SparseGaussianAdam.step(max_norm=)); `last_grad_norm` is the norm of the
-        latest step before clipping, a device scalar."""
+        latest step before clipping, a device scalar: infinite or NaN for a step that was skipped
+        (infinite for a replayed view that outgrew its graph)."""
         self.device = torch.device(device)
         self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None

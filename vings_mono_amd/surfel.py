@@ -539,7 +539,8 @@ class SparseGaussianAdam(torch.optim.Adam):
         groups, scaled by min(1, max_norm / (norm + 1e-6)) inside the update (the .grad tensors
         are not written), and the norm before clipping is returned as a device scalar.  A norm
         that is infinite or NaN skips the step: parameters and moments stay
-        (vings_sparse_adam_clipped).  Without max_norm nothing is returned."""
+        (vings_sparse_adam_clipped).  A step that the guard drops returns infinity, whatever its
+        gradients hold.  Without max_norm nothing is returned."""
         L = _lib.lib()
         _lib.require_gpu_tensor(visibility, "visibility")
         vis = visibility.reshape(-1).contiguous()

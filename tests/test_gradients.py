@@ -639,6 +639,25 @@ def test_compact_exchange_refuses_clipping():
         mapper.fused_view(None, None, None, None, reducer=Reducer())
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=gpu)])
+def test_forward_mode_tangents_are_refused(device):
+    """They would be lost: kernels that take addresses see the values alone."""
+    fwd = torch.autograd.forward_ad
+    with fwd.dual_level():
+        for leaf in (False, True):
+            plain = torch.ones(4, device=device)
+            dual = fwd.make_dual(torch.ones(4, device=device, requires_grad=leaf), plain.clone())
+            calls = [lambda: gradients.global_norm([plain, dual]), lambda: gradients.global_norm(dual),
+                     lambda: gradients.clip_by_global_norm([dual], 1.0)]
+            if device != "cpu":                      # (there the gradients are refused before the results)
+                calls.append(lambda: gradients.clip_by_global_norm([plain], 1.0, out=[dual]))
+            for call in calls:
+                with pytest.raises(_lib.VingsError, match="tangent"):
+                    call()
+                with torch.no_grad(), pytest.raises(_lib.VingsError, match="tangent"):
+                    call()
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(_lib.VingsError):
         gradients.global_norm([torch.ones(3)])

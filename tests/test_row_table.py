@@ -468,6 +468,36 @@ def test_a_run_of_them_together(captured):
     assert abs(float(gradients.global_norm([table.grad, bias.grad])) - norms[-1]) <= 2 * U * norms[-1]
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_tangents_are_refused(device, leaf):
+    """They would be lost: kernels that take addresses see the values alone."""
+    fwd = torch.autograd.forward_ad
+    ids = torch.zeros(3, dtype=torch.int64, device=device)
+    with fwd.dual_level():
+        dual = fwd.make_dual(torch.ones((4, 2), device=device, requires_grad=leaf), torch.ones((4, 2), device=device))
+        for call in (lambda: row_table.lookup_rows(dual, ids), lambda: row_table.lookup_rows_backward(dual[:3], ids, 5)):
+            with pytest.raises(_lib.VingsError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(_lib.VingsError, match="tangent"):
+                call()
+
+
+@gpu
+def test_forward_mode_tangent_of_the_incoming_gradient_is_refused():
+    """A tangent that first appears in the backward pass; without one an open level changes nothing."""
+    fwd = torch.autograd.forward_ad
+    ids = make_ids(60, 9, "uniform")
+    table = rand((9, 4), seed=1).requires_grad_()
+    weight = rand((60, 4), seed=2)
+    with fwd.dual_level():
+        (row_table.lookup_rows(table, ids) * weight).sum().backward()
+        check_backward(weight, ids, 9, 1.0, table.grad, torch.bincount(ids, minlength=9) > 0)
+        loss = (row_table.lookup_rows(table, ids) * fwd.make_dual(weight, torch.ones_like(weight))).sum()
+        with pytest.raises(_lib.VingsError, match="tangent"):
+            loss.backward()
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(_lib.VingsError):
         row_table.lookup_rows(torch.ones((3, 2)), torch.zeros(1, dtype=torch.int64))

@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # VINGS_HIP_LIB points at an alternative build of the same library (kernel A/B experiments)
@@ -185,6 +186,17 @@ def on_device(device):
     if device.index is None or device.index == torch._C._cuda_getDevice():
         return _CURRENT
     return torch.cuda.device(device)
+
+
+def refuse_tangents(tensors, what):
+    """Kernels that take addresses see a tensor's values alone: a forward-mode tangent would be
+    lost without a word."""
+    if forward_ad._current_level < 0:                # no dual level is open
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise VingsError(f"{what} carries a forward-mode tangent, which this operator does not propagate; "
+                             "pass torch.autograd.forward_ad.unpack_dual(t).primal for the values alone")
 
 
 def require_gpu_tensor(t, name, dtype=None):

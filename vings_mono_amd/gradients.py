@@ -7,7 +7,8 @@ scripts/frontend/modules/clipping.py).
 writing them, pass `max_norm` to `surfel.SparseGaussianAdam.step`.
 
 Everything stays on the device and on the current stream: nothing synchronises (except
-`error_if_nonfinite`), so the calls can be captured into a graph.
+`error_if_nonfinite`), so the calls can be captured into a graph.  The calls stand outside
+autograd: a norm carries no gradient, and forward-mode tangents are refused.
 """
 import array
 import operator
@@ -47,6 +48,7 @@ class TensorList:
         self.tensors = tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         if not tensors:
             raise VingsError(f"{what}: no tensors given")
+        _lib.refuse_tangents(tensors, what)
         self.device = tensors[0].device
         types = list(map(_dtype, tensors))
         kinds = set(types)
@@ -101,8 +103,8 @@ def norm_and_workspace(nbytes, dev):
 def global_norm(tensors, norm_type=2.0):
     """Norm over all elements of `tensors` (a tensor or a sequence; float32, bfloat16 and float16
     may be mixed) as a float32 scalar on their device: the 2-norm, or the largest magnitude for
-    norm_type=inf.  Sums are held in 64 bits: no overflow below the largest float32 norm.  A
-    tensor given twice counts twice."""
+    norm_type=inf.  It carries no gradient, whatever the tensors require.  Sums are held in 64
+    bits: no overflow below the largest float32 norm.  A tensor given twice counts twice."""
     kind = _kind(norm_type)
     g = TensorList(tensors, "global_norm")
     L, numels = _lib.lib(), _address(g.numels)
@@ -118,9 +120,10 @@ def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
     """Scales `tensors` by min(1, max_norm / (norm + 1e-6)), norm = global_norm(tensors), and
     returns the norm.  In place, or into `out`: as many tensors of the same shapes and strides,
     each of its input's type or float32 (clipped float32 gradients of a bfloat16 backward pass),
-    overlapping nothing else of the call.  In place a gradient that is short enough is left
-    unwritten.  NaN gradients give a NaN norm and NaN results; an infinite norm gives zeros (and
-    NaN where the gradient itself is infinite), or NaN if max_norm is infinite too."""
+    overlapping nothing else of the call.  Autograd does not see the scaling.  In place a gradient
+    that is short enough is left unwritten.  NaN gradients give a NaN norm and NaN results; an
+    infinite norm gives zeros (and NaN where the gradient itself is infinite), or NaN if max_norm is
+    infinite too."""
     kind = _kind(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

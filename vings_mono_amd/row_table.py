@@ -28,6 +28,7 @@ def _rows_2d(t):
 
 
 def _check(t, ids, name):
+    _lib.refuse_tangents((t,), name)
     if t.get_device() != ids.get_device() or t.get_device() < 0:
         _lib.require_gpu_tensor(t, name)
         _lib.require_gpu_tensor(ids, "ids")
@@ -92,6 +93,7 @@ class _LookupRows(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         ids, = ctx.saved_tensors
+        _lib.refuse_tangents((g,), "the incoming gradient")
         rows = torch.empty((ctx.num_rows, g.shape[-1]), dtype=g.dtype, device=g.device)
         _lookup_backward(g, ids, ctx.num_rows, ctx.scale, ctx.padding_id, rows, ctx.touched, True)
         if ctx.touched is not None:
@@ -101,7 +103,7 @@ class _LookupRows(torch.autograd.Function):
 
 def lookup_rows(table, ids, scale=1.0, padding_id=None, touched=None):
     """scale * table[ids] as a tensor of shape ids.shape + (D,) and table's type; differentiable
-    in table (once).
+    in table (once, in reverse mode; forward-mode tangents are refused).
 
     table [V, D] float32 / bfloat16 / float16, its rows may lie in a wider array; ids int32 or
     int64 of any shape.  An id outside [0, V) names no row: zeros, and no gradient (-1 for a splat

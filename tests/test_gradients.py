@@ -630,6 +630,20 @@ def test_a_dropped_view_step_reports_no_norm():
     assert 0 < float(mapper.last_grad_norm) < math.inf
 
 
+@gpu
+def test_step_counts_as_written():
+    """Parameters and moments that autograd saved before a clipped step are noticed in the backward pass."""
+    ps, gs, ms, vs, vis = adam_state(100, (3, 1), seed=6)
+    opt, params = optimizer(ps, gs, ms, vs)
+    arrays = [t for p in params for t in (p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq"])]
+    versions = [t._version for t in arrays]
+    product = params[0] * params[0]
+    opt.step(vis, 100, max_norm=1.0)
+    assert all(t._version > v for t, v in zip(arrays, versions))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+
+
 def test_compact_exchange_refuses_clipping():
     class Reducer:
         world, compact, n = 2, True, 4

@@ -641,4 +641,6 @@ class SparseGaussianAdam(torch.optim.Adam):
                 ptr(vis), N, max_norm, ptr(norm), ws, nbytes,
                 None if guard is None else guard[0], 0 if guard is None else int(guard[1]),
                 stream_ptr(dev)), "vings_sparse_adam_clipped")
+        # (the .grad tensors are only read; a step skipped on the device counts as written too)
+        torch.autograd.graph.increment_version(params + ms + vs)
         return norm

@@ -545,3 +545,14 @@ def test_backward_arguments():
         assert call(**change) != 0 and text in _error(), change
     assert size(0, 9, 4, 0) == 0 and size(10, 9, 4, 9) == 0 and size(10, 0, 4, 0) == 0
     assert size(10, 5000, 4, 0) >= 80 and size(100000, 5000, 4, 0) >= 4 * 4 * 100000   # both sides of the passes
+
+
+@host_only
+@pytest.mark.parametrize("n,rows,cols,ty", [(1000000, 257, 64, 0), (4000000, 257, 64, 0), (4190000, 260, 90, 1),
+                                            (300000, 600, 30, 0), (1000000, 1000, 12, 0), (100000, 4095, 16, 2)])
+def test_workspace_of_numbered_runs(n, rows, cols, ty):
+    """A tile of 1024 ids leaves min(rows, 1024) partial rows at most; beside those stand two bytes a
+    tile and row."""
+    size = _lib.lib().vings_row_lookup_backward_workspace_bytes
+    tiles = -(-n // 1024)
+    assert 0 < size(n, rows, cols, ty) <= tiles * (4 * min(rows, 1024) * cols + 2 * rows) + 4096

@@ -365,6 +365,9 @@ struct Segments {
     bool by_row;
 };
 
+// Partial rows that a tile of the few-rows form leaves with numbered runs, at most.
+__host__ __device__ __forceinline__ int64_t tile_runs(int64_t rows) { return rows < kTileIds ? rows : kTileIds; }
+
 // Sums of the runs of equal keys among a workgroup's `len` sorted positions.  skey[1 .. len]: the
 // keys, skey[0] and skey[len + 1] those before and behind them (kNoKey where there are none);
 // load(i): this lane's columns of the gradient row at position i.  Calls write(row, sum) for runs
@@ -701,7 +704,7 @@ __global__ __launch_bounds__(kTileThreads) void row_tile_kernel(Segments S, cons
     const char* from = reinterpret_cast<const char*>(grad + first * S.ld + c);
     // where a sum goes: a row of the result, or a partial row (see Segments)
     char* to = ALONE ? reinterpret_cast<char*>(out + c)
-                     : reinterpret_cast<char*>(S.partial + (S.by_row ? tile : tile * kTileIds) * S.D + c);
+                     : reinterpret_cast<char*>(S.partial + (S.by_row ? tile : tile * tile_runs(S.rows)) * S.D + c);
     const uint32_t step = (uint32_t)S.D * (ALONE ? (uint32_t)sizeof(O) : S.by_row ? 4u * (uint32_t)tiles : 4u);
     sum_runs<T, V, kTileThreads>(
         S, n_runs, skey, len, col_ok, sh, [&](int i) { return *reinterpret_cast<const vec*>(from + spos[i]); },
@@ -744,7 +747,7 @@ __global__ __launch_bounds__(THREADS) void row_tile_join_kernel(Segments S, cons
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t at = min(t0 + u * n_groups, tiles - 1);
-            const int64_t slot = S.by_row ? row * tiles + at : at * kTileIds + (k[u] ? k[u] - 1 : 0u);
+            const int64_t slot = S.by_row ? row * tiles + at : at * tile_runs(S.rows) + (k[u] ? k[u] - 1 : 0u);
 #pragma unroll
             for (int i = 0; i < V; ++i) f[u][i] = part[slot * S.D + i];
         }
@@ -799,7 +802,7 @@ SegmentPlan plan_segments(int64_t N, int64_t rows, int64_t D, int type) {
     const int64_t tiles = (N + kTileIds - 1) / kTileIds;
     p.by_row = rows <= 256;
     const int64_t passes = rows < kRadix ? 1 : 2;
-    const int64_t split = 2 * tiles * std::min<int64_t>(rows, kTileIds) * D * 4 + (p.by_row ? 0 : 64 * tiles * rows);
+    const int64_t split = 2 * tiles * tile_runs(rows) * D * 4 + (p.by_row ? 0 : 64 * tiles * rows);
     p.few = rows <= kFewRows && vectors <= 16 && tiles <= kFewTiles && tiles * rows <= (1 << 23) &&
             split <= passes * ((64 << 20) + 90 * N);
     if (p.few) {
@@ -844,7 +847,7 @@ GradWorkspace carve_grad(void* ws, const SegmentPlan& s, int64_t N, int64_t rows
     w.thist = (uint32_t*)take(tiles ? 4 * kRadix * ntiles : 0);
     w.totals = (uint32_t*)take(tiles ? 4 * kRadix : 0);
     const size_t pieces = s.pieces > 1 ? s.pieces : 0;
-    w.partial = (float*)take(sizeof(float) * pieces * (s.by_row ? rows : s.few ? kTileIds : 2) * D);
+    w.partial = (float*)take(sizeof(float) * pieces * (s.by_row ? rows : s.few ? tile_runs(rows) : 2) * D);
     w.met = (uint16_t*)take(s.few ? 2 * pieces * rows : 0);
     w.bytes = off;
     return w;

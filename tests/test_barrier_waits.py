@@ -1,7 +1,9 @@
 """The assembly hipcc writes for the tensor and row-table kernels: on every path to a workgroup
 barrier the wave has waited for its LDS stores.  hipcc 7.2 leaves that wait out in front of a
-barrier at a loop's head that the back edge reaches with stores under way; the kernels place their
-barriers elsewhere, and this test sees to it that it stays so."""
+barrier at a loop's head that the back edge reaches with stores under way.  The training operators'
+kernels place their plain barriers behind the stores (a vote such as __syncthreads_or may stand at a
+head: it has an LDS store and a barrier behind it of its own); the assembly of every source is
+searched for barriers without the wait."""
 import os
 import re
 import shutil
@@ -71,3 +73,26 @@ def test_every_barrier_waits_for_lds_stores(source, tmp_path):
     asm = out.read_text()
     assert asm.count("s_barrier") > 0
     assert barriers_without_wait(asm) == []
+
+
+STRICT = ("surfel_project", "sparse_adam", "splat_step", "loop_rectify", "splat_knn")     # as in the Makefile
+OTHERS = sorted(f[:-4] for f in os.listdir(CSRC) if f.endswith(".hip"))
+OTHERS = [s for s in OTHERS if s not in ("row_table", "grad_norm", "sparse_adam")]
+
+
+@pytest.mark.skipif(shutil.which(HIPCC) is None, reason="no hipcc")
+@pytest.mark.parametrize("source", OTHERS)
+def test_every_barrier_of_the_other_sources_waits_for_lds_stores(source, tmp_path):
+    out = tmp_path / "kernels.s"
+    strict = ["-ffp-contract=off"] if source in STRICT else []
+    subprocess.run([HIPCC, *FLAGS, *strict, "-o", str(out), os.path.join(CSRC, source + ".hip")], check=True,
+                   stderr=subprocess.DEVNULL)
+    assert barriers_without_wait(out.read_text()) == []
+
+
+@pytest.mark.parametrize("source", ["row_table.hip", "grad_norm.hip", "grad_norm.hpp", "sparse_adam.hip", "radix_sort.hpp"])
+def test_no_loop_of_the_training_operators_begins_with_a_barrier(source):
+    text = open(os.path.join(CSRC, source)).read()
+    heads = re.findall(r"\b(?:for|while) \([^{}]*\) \{\s*__syncthreads\(\);", text) + \
+        re.findall(r"\bdo \{\s*__syncthreads\(\);", text)
+    assert heads == []

@@ -448,6 +448,8 @@ __device__ __forceinline__ void sum_runs(const Segments& S, uint32_t limit, cons
 #pragma unroll
     for (int k = 0; k < V; ++k) sh.val[k * THREADS + l] = acc[k];
     sh.open[l] = open;
+    // (the vote at the loop's head goes through an LDS store of its own and a barrier behind that:
+    // the wait for it there covers the stores of the round before)
     for (int s = 1; s < n_groups; s <<= 1) {
         const int q = l - (s << S.lg);
         const bool add = open && q >= 0;
@@ -577,8 +579,8 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) sval[i * 256 + threadIdx.x] = acc[i];
+    __syncthreads();
     for (int s = n_groups >> 1; s > 0; s >>= 1) {
-        __syncthreads();
         if (g < s) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -586,6 +588,7 @@ __global__ __launch_bounds__(256) void row_join_kernel(Segments S, O* __restrict
                 sval[i * 256 + threadIdx.x] = acc[i];
             }
         }
+        __syncthreads();                              // (behind the stores, see row_tile_kernel)
     }
     if (g == 0 && col_ok) {
         write_scaled<O, V>(out + (int64_t)k * S.D + c, acc, S.scale);

@@ -75,6 +75,17 @@ def test_every_barrier_waits_for_lds_stores(source, tmp_path):
     assert barriers_without_wait(asm) == []
 
 
+@pytest.mark.skipif(shutil.which(HIPCC) is None, reason="no hipcc")
+@pytest.mark.parametrize("source", ["grad_norm", "sparse_adam"])
+def test_no_kernel_spills_to_scratch(source, tmp_path):
+    out = tmp_path / "kernels.s"
+    strict = ["-ffp-contract=off"] if source in STRICT else []
+    subprocess.run([HIPCC, *FLAGS, *strict, "-o", str(out), os.path.join(CSRC, source + ".hip")], check=True,
+                   stderr=subprocess.DEVNULL)
+    sizes = re.findall(r"\.amdhsa_kernel (\S+).*?\.amdhsa_private_segment_fixed_size (\d+)", out.read_text(), re.S)
+    assert sizes and [kernel for kernel, size in sizes if size != "0"] == []
+
+
 STRICT = ("surfel_project", "sparse_adam", "splat_step", "loop_rectify", "splat_knn")     # as in the Makefile
 OTHERS = sorted(f[:-4] for f in os.listdir(CSRC) if f.endswith(".hip"))
 OTHERS = [s for s in OTHERS if s not in ("row_table", "grad_norm", "sparse_adam")]

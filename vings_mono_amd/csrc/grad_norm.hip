@@ -129,106 +129,66 @@ __device__ __forceinline__ double range_norm(const TensorTable<CAP, OUT>& T, uin
 
 // The wider side sets the vector: 16 bytes of it per lane, so that its accesses are contiguous
 // over the lanes (16-bit gradients into float32: loads of 8 bytes).
-constexpr int kHeld = kChunk / 64;          // words a lane holds of a chunk, at most
-template <typename T, typename O> struct Scale {
-    static constexpr int V = Elem<O>::kVec, R = kChunk / (64 * V);
+template <typename T, typename O>
+__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t off, int64_t numel,
+                                            float coef) {
+    constexpr int V = Elem<O>::kVec, R = kChunk / (64 * V);
     typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     typedef typename Elem<O>::vec ovec;
-
-    static __device__ __forceinline__ void put(O* q, int r, const vec& x, float coef) {
+    const T* p = (const T*)in + off;
+    O* q = (O*)out + off;
+    const int lane = threadIdx.x & 63;
+    const int64_t n = numel - off;
+    auto put = [&](int r, const vec& x) {
         ovec o;
 #pragma unroll
         for (int k = 0; k < V; ++k) o[k] = (O)((float)x[k] * coef);
-        *(ovec*)(q + (r * 64 + (threadIdx.x & 63)) * V) = o;
+        *(ovec*)(q + (r * 64 + lane) * V) = o;
+    };
+    vec v[R];
+    if (n >= kChunk) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = *(const vec*)(p + (r * 64 + lane) * V);
+#pragma unroll
+        for (int r = 0; r < R; ++r) put(r, v[r]);
+        return;
     }
-    // a whole chunk, by way of the caller's registers: W words a vector
-    static constexpr int W = V * sizeof(T) / 4;
-    typedef uint32_t words __attribute__((ext_vector_type(W)));
-    typedef T plain __attribute__((ext_vector_type(V)));
-    static __device__ __forceinline__ void load(const void* in, int64_t off, uint32_t held[kHeld]) {
-        const T* p = (const T*)in + off;
+    // whole vectors, all in flight, then the up to V - 1 elements behind them
+    const int whole = (int)n / V, at = whole * V + lane;
+    const T rest = p[min(at, (int)n - 1)];
+    if (whole > 0) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const vec x = *(const vec*)(p + (r * 64 + (threadIdx.x & 63)) * V);
-            const words y = __builtin_bit_cast(words, (plain)x);
-#pragma unroll
-            for (int k = 0; k < W; ++k) held[r * W + k] = y[k];
-        }
+        for (int r = 0; r < R; ++r) v[r] = *(const vec*)(p + min(r * 64 + lane, whole - 1) * V);
     }
-    static __device__ __forceinline__ void store(void* out, int64_t off, const uint32_t held[kHeld], float coef) {
-        O* q = (O*)out + off;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            words y;
-#pragma unroll
-            for (int k = 0; k < W; ++k) y[k] = held[r * W + k];
-            put(q, r, __builtin_bit_cast(plain, y), coef);
-        }
-    }
-    // n < kChunk elements: whole vectors, all in flight, then the up to V - 1 elements behind them
-    static __device__ __forceinline__ void part(const void* in, void* out, int64_t off, int n, float coef) {
-        const T* p = (const T*)in + off;
-        O* q = (O*)out + off;
-        const int lane = threadIdx.x & 63, whole = n / V, at = whole * V + lane;
-        const T rest = p[min(at, n - 1)];
-        vec v[R];
-        if (whole > 0) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) v[r] = *(const vec*)(p + min(r * 64 + lane, whole - 1) * V);
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r * 64 + lane < whole) put(q, r, v[r], coef);
-        if (at < n) q[at] = (O)((float)rest * coef);
-    }
-};
-
-// Calls f with the Scale of a tensor's types.
-template <typename F>
-__device__ __forceinline__ void by_types(int type, int out_type, F f) {
-    if (type == ELEM_F32) f(Scale<float, float>());
-    else if (type == ELEM_BF16 && out_type == ELEM_F32) f(Scale<__bf16, float>());
-    else if (type == ELEM_BF16) f(Scale<__bf16, __bf16>());
-    else if (out_type == ELEM_F32) f(Scale<_Float16, float>());
-    else f(Scale<_Float16, _Float16>());
+    for (int r = 0; r < R; ++r)
+        if (r * 64 + lane < whole) put(r, v[r]);
+    if (at < (int)n) q[at] = (O)((float)rest * coef);
 }
 
-// Scales chunks [lo, hi); norm_of() gives the coefficient.  A wave's first chunk is loaded before
-// that, so that its way from memory and the join of the partial results take their time together
-// (clip of 300 k splats 18.6 -> 17.6 us).  A gradient that is already short enough stays as it is: in
-// place, nothing is written.
+// A gradient that is already short enough stays as it is: in place, nothing is read or written.
 // The chunks are taken from the last to the first: what the norm read last is still in the cache.
-template <int CAP, typename F>
+// (A wave's first chunk loaded ahead of the norm's join was waited for at once, the loads being in
+// branches on the tensor's type, and cost 12 bytes of scratch: kernel at 300 k splats 8.8 us with it,
+// 8.5 without, 5 M splats 145 and 143 us in all, 60 tensors 279 and 281.)
+template <int CAP>
 __device__ __forceinline__ void range_scale(const TensorTable<CAP, true>& T, uint32_t lo,
-                                            uint32_t hi, int waves, F coef_of) {
+                                            uint32_t hi, int waves, float coef) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool any = hi > lo + w;                 // (every wave takes part in the join)
-    uint32_t c = any ? hi - 1 - w : 0;
-    int t = any ? tensor_of(T, c) : 0;
-    uint32_t held[kHeld];
-    int64_t off = any ? (int64_t)(c - T.first[t]) * kChunk : 0;
-    bool holds = any && T.n[t] - off >= kChunk;
-    if (holds)
-        by_types(T.type[t], T.out_type[t], [&](auto s) {
-            decltype(s)::load(T.in[t], off, held);
-        });
-    const float coef = coef_of();
-    if (!any) return;
+    if (hi <= lo + w) return;
+    uint32_t c = hi - 1 - w;
+    int t = tensor_of(T, c);
     for (;;) {
         while (c < T.first[t]) --t;
         if (coef != 1.0f || T.in[t] != T.out[t]) {
-            off = (int64_t)(c - T.first[t]) * kChunk;
-            by_types(T.type[t], T.out_type[t], [&](auto s) {
-                typedef decltype(s) S;
-                if (T.n[t] - off < kChunk) {
-                    S::part(T.in[t], T.out[t], off, (int)(T.n[t] - off), coef);
-                    return;
-                }
-                if (!holds) S::load(T.in[t], off, held);
-                S::store(T.out[t], off, held, coef);
-            });
+            const int64_t off = (int64_t)(c - T.first[t]) * kChunk;
+            const int ty = T.type[t], ot = T.out_type[t];
+            if (ty == ELEM_F32) chunk_scale<float, float>(T.in[t], T.out[t], off, T.n[t], coef);
+            else if (ty == ELEM_BF16 && ot == ELEM_F32) chunk_scale<__bf16, float>(T.in[t], T.out[t], off, T.n[t], coef);
+            else if (ty == ELEM_BF16) chunk_scale<__bf16, __bf16>(T.in[t], T.out[t], off, T.n[t], coef);
+            else if (ot == ELEM_F32) chunk_scale<_Float16, float>(T.in[t], T.out[t], off, T.n[t], coef);
+            else chunk_scale<_Float16, _Float16>(T.in[t], T.out[t], off, T.n[t], coef);
         }
-        holds = false;
         if (c < lo + waves) break;
         c -= waves;
     }
@@ -272,13 +232,11 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(TensorTable<CAP, true> 
     __shared__ double scratch[16];
     __shared__ TensorTable<CAP, true> T;
     copy_table(args, T);
+    const float v = norm_of_partials<KIND>(partial, n_partial, scratch);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
     uint32_t lo, hi;
     block_range(T.first[T.count], lo, hi);
-    range_scale(T, lo, hi, 4, [&] {
-        const float v = norm_of_partials<KIND>(partial, n_partial, scratch);
-        if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
-        return clip_coefficient(v, max_norm);
-    });
+    range_scale(T, lo, hi, 4, clip_coefficient(v, max_norm));
 }
 
 // Norm and scaling of a few chunks by one workgroup.
@@ -292,11 +250,9 @@ __global__ __launch_bounds__(1024) void clip_one_block_kernel(TensorTable<CAP, t
     const int waves = blockDim.x >> 6;
     const uint32_t hi = T.first[T.count];
     const double s = norm_join_block<KIND>(range_norm<KIND>(T, 0u, hi, waves), scratch);
-    range_scale(T, 0u, hi, waves, [&] {
-        const float v = (float)(KIND == NORM_2 ? sqrt(s) : s);
-        if (threadIdx.x == 0) *norm = v;
-        return clip_coefficient(v, max_norm);
-    });
+    const float v = (float)(KIND == NORM_2 ? sqrt(s) : s);
+    if (threadIdx.x == 0) *norm = v;
+    range_scale(T, 0u, hi, waves, clip_coefficient(v, max_norm));
 }
 
 __global__ void norm_of_nothing_kernel(float* norm) { *norm = 0.0f; }

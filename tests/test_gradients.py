@@ -644,6 +644,54 @@ def test_step_counts_as_written():
         product.sum().backward()
 
 
+@gpu
+def test_fused_and_captured_view_steps_apply_the_clipped_gradient():
+    """Their moments, not only the norm they report: this Adam moves parameters alike whatever the
+    gradients' scale.  From equal maps the moments of a step on g * c are c and c^2 times those on g;
+    two backward passes differ by 1e-4 of their norm (the order of the blend's atomics), here an
+    eighth and a 64th are told from 1.  The captured step (second call) starts from maps that
+    moved apart by such differences; without the coefficient its first moments would be 4.7 times
+    those of the eager one."""
+    intr = synth.intrinsic_for(160, 96)
+    raw = synth.make_splats(2000, 160, 96)
+    eye = torch.eye(4, device=DEV)
+    with torch.no_grad():
+        gtp = harness.render({k: v.to(DEV) for k, v in synth.perturb_splats(raw).items()}, eye, intr)
+    settings, R = harness.view_settings(eye, intr), torch.eye(3)
+
+    def mapper(max_norm):
+        gt = {"rgb": gtp["rgb"].clone(), "depth": gtp["depth"].clone(), "depth_cov": torch.ones_like(gtp["depth"])}
+        return harness.SurfelMapper(raw, DEV, max_grad_norm=max_norm), gt
+
+    def moments(m, k):
+        st = m.optimizer.state[m.params[k]]
+        return st["exp_avg"].double(), st["exp_avg_sq"].double()
+
+    def near(a, b, tol):
+        assert float(b.norm()) > 0 and float((a - b).norm()) <= tol * float(b.norm())
+
+    loose, gt = mapper(1e9)
+    loose.fused_view(settings, intr, gt, R)
+    full = float(loose.last_grad_norm)
+    coef = (full / 8) / (full + 1e-6)
+    fused, gf = mapper(full / 8)
+    graphed, gg = mapper(full / 8)
+    fused.fused_view(settings, intr, gf, R)
+    graphed.fused_view_graphed("kf", settings, intr, gg, R)
+    for m in (fused, graphed):
+        for k in m.NAMES:
+            (a1, a2), (b1, b2) = moments(m, k), moments(loose, k)
+            near(a1, coef * b1, 1e-2)
+            near(a2, coef * coef * b2, 2e-2)
+    fused.fused_view(settings, intr, gf, R)
+    graphed.fused_view_graphed("kf", settings, intr, gg, R)
+    assert graphed._view_graphs["kf"]["graph"] is not None
+    for k in fused.NAMES:
+        (a1, a2), (b1, b2) = moments(graphed, k), moments(fused, k)
+        near(a1, b1, 0.1)
+        near(a2, b2, 0.2)
+
+
 def test_compact_exchange_refuses_clipping():
     class Reducer:
         world, compact, n = 2, True, 4

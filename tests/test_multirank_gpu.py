@@ -95,6 +95,35 @@ def test_multi_rank_view_steps(tmp_path, world):
         assert float((s0["autograd"][k] - s0["fused"][k]).abs().max()) <= 1e-4 * scale, k
 
 
+def test_clipped_view_steps_of_two_ranks(tmp_path):
+    """max_grad_norm with the planar exchange: the norm is that of the summed gradient, every rank
+    holds the same one, and the replicas stay bit-identical; the compact exchange refuses."""
+    out = str(tmp_path / "state")
+    env = dict(os.environ, MASTER_ADDR="127.0.0.1", OMP_NUM_THREADS="2")
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "2",
+           "--master-addr", "127.0.0.1", "--master-port", str(_free_port()),
+           os.path.join(HERE, "_clip_worker.py"), out]
+    res = subprocess.run(cmd, env=env, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stdout[-2000:] + res.stderr[-4000:]
+    a, b = (torch.load(out + f".rank{r}.pt", weights_only=True) for r in range(2))
+    assert a["refused"] and b["refused"] and a["full"] == b["full"] > 0
+    for step in ("fused0", "fused1", "autograd0", "autograd1"):
+        assert torch.equal(a[step]["norm"], b[step]["norm"]), step
+        for part in ("params", "m", "v"):
+            for k in a[step][part]:
+                assert torch.equal(a[step][part][k], b[step][part][k]), (step, part, k)
+    # from equal maps the moments of a step on g * c are c and c^2 times those on g; two runs of a
+    # backward pass differ by 1e-4 of their norm
+    coef = (a["full"] / 8) / (a["full"] + 1e-6)
+    for step in ("fused0", "autograd0"):
+        assert abs(float(a[step]["norm"]) - a["full"]) <= 1e-3 * a["full"], step
+        for part, factor, tol in (("m", coef, 1e-2), ("v", coef * coef, 2e-2)):
+            for k in a[step][part]:
+                want = a["loose"][part][k].double() * factor
+                assert float(want.norm()) > 0
+                assert float((a[step][part][k].double() - want).norm()) <= tol * float(want.norm()), (step, part, k)
+
+
 def test_bench_starts_its_own_ranks():
     """`python bench.py --gpus 2` with no launcher around it (the way the driver starts the
     bench): the process starts its two ranks itself and hands on rank 0's line."""

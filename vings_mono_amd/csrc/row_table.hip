@@ -30,7 +30,7 @@
 // Sums are float32: at most 64 terms in a row in a lane group, then the scan, then the partial rows
 // of a run dealt out over the lane groups of its join; the result is scaled and rounded once.
 // Measured: 16381 ids into 32768 rows of 2048 bfloat16 in 58 us, of which the two sorting launches
-// 26 (they clear 134 MB meanwhile, at 5.3 TB/s), segments 25, join 5; a million ids into 80 rows of
+// 24 (they clear 134 MB meanwhile, at 5.6 TB/s), segments 24, join 6; a million ids into 80 rows of
 // 12 float32 in 23 us (local sums 19: 2 us of latency for each of ids, ranking and rows, then 56 MB
 // at 4.7 TB/s; join 4).
 //

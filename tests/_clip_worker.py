@@ -1,5 +1,5 @@
 """Worker of the clipped view steps in tests/test_multirank_gpu.py: one rank of a job whose ranks
-share the GPU of the test box and exchange over gloo."""
+share one GPU and exchange over gloo."""
 import os
 import sys
 
